@@ -165,6 +165,97 @@ int kq_step_run(kq_step *step, int64_t pos, int flags);
 int kq_step_trace(kq_step *step, uint64_t *trace, size_t words);
 int kq_step_destroy(kq_step *step);
 
+/* ---- paged key-value cache (serving many sequences of different lengths) ----
+ * The keys and values of all sequences share two pools of f16 pages, page p of
+ * a pool at pool + p * page_ld elements, each [kv_heads][page_size][head_dim].
+ * A block table names each sequence's pages: slot j of sequence b lies in page
+ * table[b * table_ld + j / page_size], row j % page_size.  Entries behind the
+ * last used slot are not read.  kq_kv_create keeps the pools' addresses, not
+ * the memory; the pools must outlive the handle, and the context the handle.
+ *   head_dim 64, 128 or 256; page_size a multiple of 16 up to 1024; page_ld a
+ *   multiple of 8; pools 16-byte aligned; 1 to 16 query heads per kv head;
+ *   batch up to 65535.
+ * All pointers below are device pointers on the context's device; calls are
+ * queued on its stream.  lens, slots, positions and table entries are read on
+ * the device, so a captured graph replays with their values of the moment.
+ * One that lies outside its bounds is not followed: nothing is read or written
+ * there, and the next kq_ctx_synchronize reports KQ_ERR_INVALID_ARG.
+ * No reference counterpart: its cache is one contiguous block per sequence
+ * (kv_cache.rs:57-80). */
+typedef struct kq_kv kq_kv;
+int kq_kv_create(kq_ctx *ctx, void *k_pool, void *v_pool, int64_t pages, int64_t page_ld, int page_size, int kv_heads,
+                 int head_dim, kq_kv **out);
+int kq_kv_destroy(kq_kv *kv);
+/* Rows of q (heads) | k (kv_heads) | v (kv_heads), ld floats apart, into the
+ * cache: row r goes to slot slots[r] of sequence seqs[r] (NULL: sequence r), k
+ * turned to position pos[r] (NULL: the slot) as in kq_dec_rope_append, with
+ * the angle reduced in 64 bits, k and v rounded to f16.  slots[r] = -1 skips
+ * the row.  q_out (NULL: not needed; it may be qkv itself with q_ld = ld)
+ * receives the turned query heads.  slot_pos [batch][kv_heads][track_ld]
+ * (NULL: not kept) receives the position of each written slot.  The slots of
+ * one call must be distinct; of two rows for one slot either may be stored,
+ * in part. */
+int kq_kv_append(kq_kv *kv, const float *qkv, int64_t ld, int64_t rows, int heads, const int32_t *seqs,
+                 const int32_t *slots, const int32_t *pos, const int32_t *table, int64_t table_ld, int64_t batch,
+                 float theta, float *q_out, int64_t q_ld, int32_t *slot_pos, int64_t track_ld);
+/* Scratch bytes of the two calls below (track_len: track_ld where mass is
+ * given, else 0); 0 for sizes that they refuse.  256-byte aligned, zero-filled
+ * before its first use (it holds arrival counters that every call leaves at
+ * zero); one scratch serves one call at a time, so graphs that may run at the
+ * same time need one each. */
+size_t kq_kv_attention_scratch(const kq_kv *kv, int64_t batch, int heads, int64_t track_len);
+/* Attention of one token per sequence over slots [0, lens[b]):
+ * out[b][h] = softmax(q[b][h] . k^T / sqrt(head_dim)) . v with grouped query
+ * heads (q turned already).  lens[b] = 0 is an idle row: out[b] is zero.
+ * mass [batch][kv_heads][track_ld] (NULL: not kept; lens[b] <= track_ld)
+ * accumulates each slot's attention weight, summed over the group's heads. */
+int kq_kv_attention(kq_kv *kv, const float *q, int64_t q_ld, float *out, int64_t out_ld, int64_t batch, int heads,
+                    const int32_t *table, int64_t table_ld, const int32_t *lens, float *mass, int64_t track_ld,
+                    void *scratch, size_t scratch_bytes);
+/* The same with the step's new token: qkv rows as in kq_kv_append; q is turned
+ * in registers (qkv is not modified), the turned k and v go to slot lens[b] - 1
+ * (lens counts the new slot), then the attention over all lens[b] slots.
+ * pos[b]: the new token's position (NULL: lens[b] - 1; they differ once slots
+ * were evicted).  The new slot's mass starts anew, and slot_pos (NULL: not
+ * kept) receives its position. */
+int kq_kv_rope_attention(kq_kv *kv, const float *qkv, int64_t ld, float *out, int64_t out_ld, int64_t batch, int heads,
+                         const int32_t *table, int64_t table_ld, const int32_t *lens, const int32_t *pos, float theta,
+                         float *mass, int32_t *slot_pos, int64_t track_ld, void *scratch, size_t scratch_bytes);
+/* Cuts sequences of more than `keep` slots down to `keep`, per kv head by
+ * accumulated attention weight: first the slots whose slot_pos is at least
+ * recent_from[b] (NULL: none is protected), then those of the greatest mass,
+ * ties to the lowest slot (NaN counts as -inf).  Attention does not depend on
+ * the order of the slots, so rows move as little as possible: the freed slots
+ * below `keep`, in ascending order, take the kept rows above it, in ascending
+ * order.  mass and slot_pos move along into mass_out and pos_out (each may be
+ * its input, or another array: [0, min(lens, keep)) of each head is written);
+ * lens_out[b] = min(lens[b], keep) (it may be lens).  Sequences that share
+ * pages must not be evicted.  scratch: kq_kv_evict_scratch bytes, 256-byte
+ * aligned, not initialised. */
+size_t kq_kv_evict_scratch(const kq_kv *kv, int64_t batch, int64_t track_ld);
+int kq_kv_evict(kq_kv *kv, int64_t batch, const int32_t *table, int64_t table_ld, const int32_t *lens,
+                int32_t *lens_out, const float *mass, const int32_t *slot_pos, float *mass_out, int32_t *pos_out,
+                int64_t track_ld, const int32_t *recent_from, int32_t keep, void *scratch, size_t scratch_bytes);
+
+/* The next token of every sequence from its logits (rows ld floats apart),
+ * given uniform random numbers u[b] in [0, 1).  With the tokens in the order
+ * (logit descending, index ascending) and weights w = e^((z - max) /
+ * temperature), each filter keeps a prefix, at least the first token:
+ *   top_k   the first top_k (<= 0: all);
+ *   top_p   of those, each whose predecessors hold less than top_p of their
+ *           weight (>= 1: all);
+ *   min_p   those with w >= min_p (w of the first is 1).
+ * tokens[b] is then the first token in index order whose cumulative weight
+ * over the kept ones exceeds u[b] times their sum.  temperature <= 0 takes the
+ * first.  Logits of -inf (and NaN) are never taken; a row without any other
+ * gives token -1.  temperature, top_k, top_p, min_p: [batch] each, or NULL (1,
+ * all, 1, 0).  prob (NULL: not needed) receives the token's share of the kept
+ * weight, kept (NULL) the number of kept tokens.  Weights are summed in 64-bit
+ * fixed point: the same call gives the same tokens.  vocab up to 393216. */
+int kq_dec_sample(kq_ctx *ctx, const float *logits, int64_t ld, int64_t batch, int64_t vocab, const float *temperature,
+                  const int32_t *top_k, const float *top_p, const float *min_p, const float *u, int32_t *tokens,
+                  float *prob, int32_t *kept);
+
 /* out[b] = table[tokens[b]] (Model::embed, model.rs:966-984); table f32 [vocab][dim]. */
 int kq_dec_embed(kq_ctx *ctx, const float *table, const int32_t *tokens, float *out, int64_t out_ld,
                  int64_t batch, int64_t dim);

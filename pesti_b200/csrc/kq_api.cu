@@ -5,9 +5,11 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <new>
 #include <string>
 #include <vector>
 
@@ -79,6 +81,12 @@ struct kq_weight {
   void* q_alloc = nullptr;
   void* d_alloc = nullptr;
   int64_t device_bytes = 0;
+};
+
+// A paged key-value cache over the caller's pools (kq_kv_*).
+struct kq_kv {
+  kq_ctx* ctx = nullptr;
+  kq::KvPool pool;
 };
 
 // A decode-step program (kq_step_*): its stages on the host, and once built,
@@ -190,10 +198,18 @@ int check_device_error(kq_ctx* ctx) {
   if (ctx->ctr) cudaMemset(ctx->ctr, 0, ctx->ctr_bytes);
   cudaDeviceSynchronize();
   cudaGetLastError();
+  if (code >= 51 && code <= 53)
+    return fail(ctx, KQ_ERR_INVALID_ARG,
+                "a paged-cache call met %s (code %d); nothing was read or written there and the call's output is "
+                "invalid",
+                code == 51   ? "a page outside the pool"
+                : code == 52 ? "a sequence length outside its block table"
+                             : "a row whose sequence or slot lies outside the block table",
+                code);
   return fail(ctx, KQ_ERR_CUDA,
               "a device-side wait gave up (code %d: 1-5 tcgen05 pipeline, 21-23 decode weight ring, "
               "27-28 batched integer-MMA ring, 31-32 tensor-parallel peer flag, 41-45 decode-step ring, "
-              "barrier or exchange); the call's output is invalid",
+              "barrier or exchange, 54 paged-attention ring); the call's output is invalid",
               code);
 }
 
@@ -309,6 +325,8 @@ int kq_ctx_create(int device, kq_ctx** out) {
   if (e == cudaSuccess) e = kq::dp4a_init_device();
   if (e == cudaSuccess) e = kq::imma_init_device();
   if (e == cudaSuccess) e = kq::dec_init_device();
+  if (e == cudaSuccess) e = kq::kv_init_device();
+  if (e == cudaSuccess) e = kq::sample_init_device();
   if (e == cudaSuccess) e = kq::kx_init_device();
   if (e == cudaSuccess) e = kq::step_init_device();
   if (e != cudaSuccess) {
@@ -1255,6 +1273,244 @@ int kq_dec_embed(kq_ctx* ctx, const float* table, const int32_t* tokens, float* 
   DeviceGuard g(ctx->device);
   ctx->launches += 1;
   return dec_status(ctx, kq::dec_embed(table, tokens, out, out_ld, batch, dim, ctx->stream), "embed");
+}
+
+// ---- paged key-value cache ----------------------------------------------------------
+
+int kq_kv_create(kq_ctx* ctx, void* k_pool, void* v_pool, int64_t pages, int64_t page_ld, int page_size, int kv_heads,
+                 int head_dim, kq_kv** out) {
+  if (check_ctx(ctx) || !out) return KQ_ERR_INVALID_ARG;
+  *out = nullptr;
+  if (!k_pool || !v_pool) return fail(ctx, KQ_ERR_INVALID_ARG, "kq_kv_create: null pool");
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256)
+    return fail(ctx, KQ_ERR_UNSUPPORTED, "kq_kv_create: head_dim %d (64, 128 or 256)", head_dim);
+  if (page_size < 16 || page_size > 1024 || page_size % 16)
+    return fail(ctx, KQ_ERR_UNSUPPORTED, "kq_kv_create: page_size %d (a multiple of 16 up to 1024)", page_size);
+  if (pages < 1 || pages > INT32_MAX || kv_heads < 1 || kv_heads > 65535 || page_ld % 8 ||
+      page_ld < (int64_t)kv_heads * page_size * head_dim || page_ld > (int64_t)1 << 38)
+    return fail(ctx, KQ_ERR_INVALID_ARG, "kq_kv_create: %lld pages %lld elements apart of %d heads x %d slots x %d",
+                (long long)pages, (long long)page_ld, kv_heads, page_size, head_dim);
+  if ((reinterpret_cast<uintptr_t>(k_pool) | reinterpret_cast<uintptr_t>(v_pool)) & 15)
+    return fail(ctx, KQ_ERR_INVALID_ARG, "kq_kv_create: the pools must be 16-byte aligned");
+  kq_kv* kv = new (std::nothrow) kq_kv;
+  if (!kv) return fail(ctx, KQ_ERR_NOMEM, "kq_kv_create: out of host memory");
+  kv->ctx = ctx;
+  kv->pool.k = k_pool;
+  kv->pool.v = v_pool;
+  kv->pool.pages = pages;
+  kv->pool.page_ld = page_ld;
+  kv->pool.page_size = page_size;
+  kv->pool.hkv = kv_heads;
+  kv->pool.hd = head_dim;
+  *out = kv;
+  return KQ_OK;
+}
+
+int kq_kv_destroy(kq_kv* kv) {
+  if (!kv) return KQ_ERR_INVALID_ARG;
+  delete kv;
+  return KQ_OK;
+}
+
+// The arguments every paged-cache call shares.
+static int kv_check(kq_kv* kv, const char* what, const int32_t* table, int64_t table_ld, int64_t batch) {
+  kq_ctx* ctx = kv->ctx;
+  if (!table || table_ld < 1 || table_ld > INT32_MAX)
+    return fail(ctx, KQ_ERR_INVALID_ARG, "%s: no block table, or rows of %lld pages", what, (long long)table_ld);
+  if (batch < 1 || batch > 65535) return fail(ctx, KQ_ERR_INVALID_ARG, "%s: batch %lld", what, (long long)batch);
+  return KQ_OK;
+}
+
+static int kv_heads_check(kq_kv* kv, const char* what, int heads) {
+  const int hkv = kv->pool.hkv;
+  if (heads < hkv || heads % hkv || heads / hkv > kq::KV_MAX_GROUP)
+    return fail(kv->ctx, KQ_ERR_UNSUPPORTED, "%s: %d query heads over %d kv heads (1 to %d per kv head)", what, heads,
+                hkv, kq::KV_MAX_GROUP);
+  return KQ_OK;
+}
+
+static bool bad_theta(float theta) { return !(theta > 0.f) || std::isinf(theta); }
+
+int kq_kv_append(kq_kv* kv, const float* qkv, int64_t ld, int64_t rows, int heads, const int32_t* seqs,
+                 const int32_t* slots, const int32_t* pos, const int32_t* table, int64_t table_ld, int64_t batch,
+                 float theta, float* q_out, int64_t q_ld, int32_t* slot_pos, int64_t track_ld) {
+  if (!kv) return KQ_ERR_INVALID_ARG;
+  kq_ctx* ctx = kv->ctx;
+  const char* what = "kq_kv_append";
+  if (!qkv || !slots) return fail(ctx, KQ_ERR_INVALID_ARG, "%s: null qkv or slots", what);
+  if (int rc = kv_check(kv, what, table, table_ld, batch)) return rc;
+  if (int rc = kv_heads_check(kv, what, heads)) return rc;
+  const int64_t hd = kv->pool.hd;
+  if (rows < 0 || rows > INT32_MAX || ld < (heads + 2 * (int64_t)kv->pool.hkv) * hd || (q_out && q_ld < heads * hd) ||
+      (slot_pos && track_ld < 1) || (!seqs && rows > batch) || bad_theta(theta))
+    return fail(ctx, KQ_ERR_INVALID_ARG, "%s: %lld rows of %lld, q rows of %lld, theta %g", what, (long long)rows,
+                (long long)ld, (long long)q_ld, (double)theta);
+  if (rows == 0) return KQ_OK;
+  kq::KvAppendArgs a;
+  a.pool = kv->pool;
+  a.qkv = qkv;
+  a.ld = ld;
+  a.rows = rows;
+  a.hq = heads;
+  a.seqs = seqs;
+  a.slots = slots;
+  a.pos = pos;
+  a.table = table;
+  a.table_ld = table_ld;
+  a.batch = batch;
+  a.log2_theta = std::log2((double)theta);
+  a.q_out = q_out;
+  a.q_ld = q_ld;
+  a.slot_pos = slot_pos;
+  a.track_ld = track_ld;
+  a.err = ctx->dev_err;
+  DeviceGuard g(ctx->device);
+  if (g.status != cudaSuccess) return cuda_fail(ctx, g.status, "cudaSetDevice");
+  const cudaError_t e = kq::kv_append(a, ctx->stream);
+  ctx->launches += e == cudaSuccess;
+  return dec_status(ctx, e, what);
+}
+
+size_t kq_kv_attention_scratch(const kq_kv* kv, int64_t batch, int heads, int64_t track_len) {
+  if (!kv || batch < 1 || batch > 65535 || heads < kv->pool.hkv || heads % kv->pool.hkv ||
+      heads / kv->pool.hkv > kq::KV_MAX_GROUP || track_len < 0)
+    return 0;
+  return kq::kv_attention_scratch_bytes(batch, heads, kv->pool.hkv, kv->pool.hd, track_len, kv->ctx->num_sms);
+}
+
+static int kv_attention_impl(kq_kv* kv, const char* what, bool rope, const float* q, int64_t q_ld, float* out,
+                             int64_t out_ld, int64_t batch, int heads, const int32_t* table, int64_t table_ld,
+                             const int32_t* lens, const int32_t* pos, float theta, float* mass, int32_t* slot_pos,
+                             int64_t track_ld, void* scratch, size_t scratch_bytes) {
+  if (!kv) return KQ_ERR_INVALID_ARG;
+  kq_ctx* ctx = kv->ctx;
+  if (!q || !out || !lens || !scratch) return fail(ctx, KQ_ERR_INVALID_ARG, "%s: null argument", what);
+  if (int rc = kv_check(kv, what, table, table_ld, batch)) return rc;
+  if (int rc = kv_heads_check(kv, what, heads)) return rc;
+  const int64_t hd = kv->pool.hd, cols = (rope ? heads + 2 * (int64_t)kv->pool.hkv : heads) * hd;
+  if (q_ld < cols || out_ld < heads * hd || ((mass || slot_pos) && (track_ld < 1 || track_ld > INT32_MAX)) ||
+      (rope && bad_theta(theta)))
+    return fail(ctx, KQ_ERR_INVALID_ARG, "%s: rows of %lld in, %lld out, %lld tracked, theta %g", what,
+                (long long)q_ld, (long long)out_ld, (long long)track_ld, (double)theta);
+  const int64_t track = mass ? track_ld : 0;
+  if (reinterpret_cast<uintptr_t>(scratch) & 255)
+    return fail(ctx, KQ_ERR_INVALID_ARG, "%s: the scratch must be 256-byte aligned", what);
+  if (scratch_bytes < kq::kv_attention_scratch_bytes(batch, heads, kv->pool.hkv, kv->pool.hd, track, ctx->num_sms))
+    return fail(ctx, KQ_ERR_SHORT_BUFFER, "%s: scratch of %zu bytes is too small", what, scratch_bytes);
+  kq::KvAttnArgs a;
+  a.pool = kv->pool;
+  a.q = q;
+  a.q_ld = q_ld;
+  a.out = out;
+  a.out_ld = out_ld;
+  a.batch = batch;
+  a.hq = heads;
+  a.table = table;
+  a.table_ld = table_ld;
+  a.lens = lens;
+  a.pos = pos;
+  a.log2_theta = rope ? std::log2((double)theta) : 0.0;
+  a.mass = mass;
+  a.slot_pos = slot_pos;
+  a.track_ld = track_ld;
+  a.scratch = scratch;
+  a.num_sms = ctx->num_sms;
+  a.err = ctx->dev_err;
+  DeviceGuard g(ctx->device);
+  if (g.status != cudaSuccess) return cuda_fail(ctx, g.status, "cudaSetDevice");
+  int launches = 0;
+  const cudaError_t e = kq::kv_attention(a, rope, &launches, ctx->stream);
+  ctx->launches += launches;
+  return dec_status(ctx, e, what);
+}
+
+int kq_kv_attention(kq_kv* kv, const float* q, int64_t q_ld, float* out, int64_t out_ld, int64_t batch, int heads,
+                    const int32_t* table, int64_t table_ld, const int32_t* lens, float* mass, int64_t track_ld,
+                    void* scratch, size_t scratch_bytes) {
+  return kv_attention_impl(kv, "kq_kv_attention", false, q, q_ld, out, out_ld, batch, heads, table, table_ld, lens,
+                           nullptr, 0.f, mass, nullptr, track_ld, scratch, scratch_bytes);
+}
+
+int kq_kv_rope_attention(kq_kv* kv, const float* qkv, int64_t ld, float* out, int64_t out_ld, int64_t batch, int heads,
+                         const int32_t* table, int64_t table_ld, const int32_t* lens, const int32_t* pos, float theta,
+                         float* mass, int32_t* slot_pos, int64_t track_ld, void* scratch, size_t scratch_bytes) {
+  return kv_attention_impl(kv, "kq_kv_rope_attention", true, qkv, ld, out, out_ld, batch, heads, table, table_ld,
+                           lens, pos, theta, mass, slot_pos, track_ld, scratch, scratch_bytes);
+}
+
+size_t kq_kv_evict_scratch(const kq_kv* kv, int64_t batch, int64_t track_ld) {
+  if (!kv || batch < 1 || batch > 65535 || track_ld < 1 || track_ld > INT32_MAX) return 0;
+  return kq::kv_evict_scratch_bytes(batch, kv->pool.hkv, track_ld);
+}
+
+int kq_kv_evict(kq_kv* kv, int64_t batch, const int32_t* table, int64_t table_ld, const int32_t* lens,
+                int32_t* lens_out, const float* mass, const int32_t* slot_pos, float* mass_out, int32_t* pos_out,
+                int64_t track_ld, const int32_t* recent_from, int32_t keep, void* scratch, size_t scratch_bytes) {
+  if (!kv) return KQ_ERR_INVALID_ARG;
+  kq_ctx* ctx = kv->ctx;
+  const char* what = "kq_kv_evict";
+  if (!lens || !lens_out || !mass || !slot_pos || !mass_out || !pos_out || !scratch)
+    return fail(ctx, KQ_ERR_INVALID_ARG, "%s: null argument", what);
+  if (int rc = kv_check(kv, what, table, table_ld, batch)) return rc;
+  if (keep < 1 || track_ld < 1 || track_ld > INT32_MAX)
+    return fail(ctx, KQ_ERR_INVALID_ARG, "%s: keep %d of %lld tracked slots", what, keep, (long long)track_ld);
+  if (reinterpret_cast<uintptr_t>(scratch) & 255)
+    return fail(ctx, KQ_ERR_INVALID_ARG, "%s: the scratch must be 256-byte aligned", what);
+  if (scratch_bytes < kq::kv_evict_scratch_bytes(batch, kv->pool.hkv, track_ld))
+    return fail(ctx, KQ_ERR_SHORT_BUFFER, "%s: scratch of %zu bytes is too small", what, scratch_bytes);
+  kq::KvEvictArgs a;
+  a.pool = kv->pool;
+  a.batch = batch;
+  a.table = table;
+  a.table_ld = table_ld;
+  a.lens = lens;
+  a.lens_out = lens_out;
+  a.mass = mass;
+  a.slot_pos = slot_pos;
+  a.mass_out = mass_out;
+  a.pos_out = pos_out;
+  a.track_ld = track_ld;
+  a.recent_from = recent_from;
+  a.keep = keep;
+  a.scratch = scratch;
+  a.err = ctx->dev_err;
+  DeviceGuard g(ctx->device);
+  if (g.status != cudaSuccess) return cuda_fail(ctx, g.status, "cudaSetDevice");
+  int launches = 0;
+  const cudaError_t e = kq::kv_evict(a, &launches, ctx->stream);
+  ctx->launches += launches;
+  return dec_status(ctx, e, what);
+}
+
+int kq_dec_sample(kq_ctx* ctx, const float* logits, int64_t ld, int64_t batch, int64_t vocab, const float* temperature,
+                  const int32_t* top_k, const float* top_p, const float* min_p, const float* u, int32_t* tokens,
+                  float* prob, int32_t* kept) {
+  if (check_ctx(ctx)) return KQ_ERR_INVALID_ARG;
+  if (!logits || !u || !tokens) return fail(ctx, KQ_ERR_INVALID_ARG, "kq_dec_sample: null logits, u or tokens");
+  if (batch < 1 || batch > 65535 || vocab < 1 || ld < vocab)
+    return fail(ctx, KQ_ERR_INVALID_ARG, "kq_dec_sample: %lld rows of %lld logits, %lld apart", (long long)batch,
+                (long long)vocab, (long long)ld);
+  if (vocab > kq::SAMPLE_MAX_VOCAB)
+    return fail(ctx, KQ_ERR_UNSUPPORTED, "kq_dec_sample: %lld logits (at most %d)", (long long)vocab,
+                kq::SAMPLE_MAX_VOCAB);
+  kq::SampleArgs a;
+  a.logits = logits;
+  a.ld = ld;
+  a.batch = batch;
+  a.vocab = (int)vocab;
+  a.temperature = temperature;
+  a.top_k = top_k;
+  a.top_p = top_p;
+  a.min_p = min_p;
+  a.u = u;
+  a.tokens = tokens;
+  a.prob = prob;
+  a.kept = kept;
+  DeviceGuard g(ctx->device);
+  if (g.status != cudaSuccess) return cuda_fail(ctx, g.status, "cudaSetDevice");
+  const cudaError_t e = kq::dec_sample(a, ctx->stream);
+  ctx->launches += e == cudaSuccess;
+  return dec_status(ctx, e, "kq_dec_sample");
 }
 
 // ---- persistent decode step ------------------------------------------------------

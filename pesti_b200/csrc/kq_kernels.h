@@ -348,6 +348,96 @@ cudaError_t dec_add(float* h, int64_t h_ld, const float* y, int64_t y_ld, int64_
 cudaError_t dec_embed(const float* table, const int* tokens, float* out, int64_t out_ld, int64_t batch, int64_t dim,
                       cudaStream_t s);
 
+// ---- paged key-value cache: kq_paged.cu ----
+// Pools of `pages` pages, page_ld elements apart, each [kv_heads][page_size][hd]
+// f16.  Slot j of sequence b lies in page table[b * table_ld + j / page_size].
+struct KvPool {
+  void* k = nullptr;
+  void* v = nullptr;
+  int64_t pages = 0, page_ld = 0;
+  int page_size = 0, hkv = 0, hd = 0;
+};
+// Per-device set-up of the paged-cache kernels (shared-memory sizes).
+cudaError_t kv_init_device();
+struct KvAppendArgs {
+  KvPool pool;
+  const float* qkv;  // row r at qkv + r * ld: q (hq heads) | k (hkv) | v (hkv)
+  int64_t ld, rows;
+  int hq;
+  const int32_t* seqs;   // [rows] sequence of each row (NULL: row r is sequence r)
+  const int32_t* slots;  // [rows] its slot, -1: the row is skipped
+  const int32_t* pos;    // [rows] its rotary position (NULL: the slot)
+  const int32_t* table;
+  int64_t table_ld, batch;
+  double log2_theta;
+  float* q_out;  // NULL: q is not needed
+  int64_t q_ld;
+  int32_t* slot_pos;  // [batch][hkv][track_ld], or NULL
+  int64_t track_ld;
+  int* err;
+};
+cudaError_t kv_append(const KvAppendArgs& a, cudaStream_t s);
+struct KvAttnArgs {
+  KvPool pool;
+  const float* q;  // token b's query heads at q + b * q_ld (rope: the fused qkv row)
+  int64_t q_ld;
+  float* out;
+  int64_t out_ld, batch;
+  int hq;
+  const int32_t* table;
+  int64_t table_ld;
+  const int32_t* lens;  // [batch] slots in use, the new one included; 0: an idle row
+  const int32_t* pos;   // rope: [batch] the new token's position (NULL: lens - 1)
+  double log2_theta;
+  float* mass;        // [batch][hkv][track_ld] accumulated weights, or NULL
+  int32_t* slot_pos;  // rope: the new slot's position is noted here, or NULL
+  int64_t track_ld;
+  void* scratch;
+  int num_sms;
+  int* err;
+};
+// head_dim 64, 128 or 256, 1 to KV_MAX_GROUP query heads per kv head.
+constexpr int KV_MAX_GROUP = 16;
+size_t kv_attention_scratch_bytes(int64_t batch, int hq, int hkv, int hd, int64_t track_len, int num_sms);
+cudaError_t kv_attention(const KvAttnArgs& a, bool rope, int* launches, cudaStream_t s);
+struct KvEvictArgs {
+  KvPool pool;
+  int64_t batch;
+  const int32_t* table;
+  int64_t table_ld;
+  const int32_t* lens;
+  int32_t* lens_out;
+  const float* mass;
+  const int32_t* slot_pos;
+  float* mass_out;
+  int32_t* pos_out;
+  int64_t track_ld;
+  const int32_t* recent_from;  // [batch], or NULL: no slot is protected
+  int32_t keep;
+  void* scratch;
+  int* err;
+};
+size_t kv_evict_scratch_bytes(int64_t batch, int hkv, int64_t track_ld);
+cudaError_t kv_evict(const KvEvictArgs& a, int* launches, cudaStream_t s);
+
+// ---- sampling: kq_sample.cu ----
+constexpr int SAMPLE_MAX_VOCAB = 393216;
+cudaError_t sample_init_device();
+struct SampleArgs {
+  const float* logits;
+  int64_t ld, batch;
+  int vocab;
+  const float* temperature;  // each [batch], or NULL: 1, 0 (off), 1, 0
+  const int32_t* top_k;
+  const float* top_p;
+  const float* min_p;
+  const float* u;
+  int32_t* tokens;
+  float* prob;    // or NULL
+  int32_t* kept;  // or NULL
+};
+cudaError_t dec_sample(const SampleArgs& a, cudaStream_t s);
+
 // ---- tensor-core (tcgen05) path: kq_mma.cu ----
 // Build the TMA descriptors of a GGUF weight (after its device arrays exist).
 bool tc_make_weight_maps(DevWeight& w);

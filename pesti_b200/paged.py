@@ -1,0 +1,206 @@
+"""Paged key-value cache on the GPU (kq_kv_*, include/pesti_decoder.h).
+
+The keys and values of all sequences live in two pools of f16 pages
+[pages][kv_heads][page_size][head_dim]; a block table names the pages of each
+sequence.  ``PagedCache`` binds a pair of pools to a context and offers what a
+decode step does with them: ``append`` rows, ``attention`` or
+``rope_attention`` of one new token per sequence, and ``evict`` by accumulated
+attention weight.  Tensors are CUDA tensors on the context's device; calls are
+queued on the context's stream and return nothing: what they write is handed in.
+"""
+from __future__ import annotations
+
+import ctypes
+
+from . import kq
+
+
+def _bind(lib: ctypes.CDLL) -> ctypes.CDLL:
+    P, I, I32, I64, F, Z = (ctypes.c_void_p, ctypes.c_int, ctypes.c_int32, ctypes.c_int64, ctypes.c_float,
+                            ctypes.c_size_t)
+    sig = {
+        "kq_kv_create": ([P, P, P, I64, I64, I, I, I, ctypes.POINTER(P)], I),
+        "kq_kv_destroy": ([P], I),
+        "kq_kv_append": ([P, P, I64, I64, I, P, P, P, P, I64, I64, F, P, I64, P, I64], I),
+        "kq_kv_attention_scratch": ([P, I64, I, I64], Z),
+        "kq_kv_attention": ([P, P, I64, P, I64, I64, I, P, I64, P, P, I64, P, Z], I),
+        "kq_kv_rope_attention": ([P, P, I64, P, I64, I64, I, P, I64, P, P, F, P, P, I64, P, Z], I),
+        "kq_kv_evict_scratch": ([P, I64, I64], Z),
+        "kq_kv_evict": ([P, I64, P, I64, P, P, P, P, P, P, I64, P, I32, P, Z], I),
+    }
+    for name, (args, res) in sig.items():
+        getattr(lib, name).argtypes = args
+        getattr(lib, name).restype = res
+    return lib
+
+
+def _invalid(message: str) -> kq.KqError:
+    return kq.KqError(kq.KQ_ERR_INVALID_ARG, message)
+
+
+class PagedCache:
+    """Two pools of pages (f16 CUDA tensors of one shape [pages][kv_heads]
+    [page_size][head_dim], contiguous within a page) as one layer's cache."""
+
+    def __init__(self, ctx: "kq.Context", k, v):
+        import torch
+        if k.dim() != 4 or k.shape != v.shape or k.stride() != v.stride():
+            raise _invalid(f"pools of shapes {tuple(k.shape)} and {tuple(v.shape)}: one shape and stride is wanted")
+        if k.dtype != torch.float16 or v.dtype != torch.float16:
+            raise _invalid(f"pools of {k.dtype} and {v.dtype}: float16 is wanted")
+        self.pages, self.kv_heads, self.page_size, self.head_dim = k.shape
+        inner = (self.page_size * self.head_dim, self.head_dim, 1)
+        if k.stride()[1:] != inner:
+            raise _invalid(f"pool strides {k.stride()}: the pages must be contiguous")
+        self.device = torch.device("cuda", ctx.device)
+        if k.device != self.device or v.device != self.device:
+            raise _invalid(f"pools on {k.device} and {v.device}, context on {self.device}")
+        self.ctx, self.k, self.v = ctx, k, v
+        self.lib = _bind(ctx.lib)
+        self._types = torch.float32, torch.int32
+        h = ctypes.c_void_p()
+        ctx.check(self.lib.kq_kv_create(ctx.handle, k.data_ptr(), v.data_ptr(), self.pages, k.stride(0),
+                                        self.page_size, self.kv_heads, self.head_dim, ctypes.byref(h)), "kq_kv_create")
+        self.handle = h
+
+    # ---- argument checks ---------------------------------------------------------------
+    def _rows(self, t, name: str, dtype, rows: int = -1):
+        """A matrix (or the flat form of one row) with unit inner stride; its row stride."""
+        if t.dtype != dtype or t.device != self.device or t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+            raise _invalid(f"{name}: {t.dtype} {tuple(t.shape)} strides {t.stride()} on {t.device}; rows of {dtype} on "
+                           f"{self.device} are wanted")
+        if 0 <= rows != t.shape[0]:
+            raise _invalid(f"{name}: {t.shape[0]} rows where {rows} are wanted")
+        return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+    def _vector(self, t, name: str, n: int):
+        """An int32 vector of n values (None stays None)."""
+        if t is None:
+            return None
+        if t.dtype != self._types[1] or t.device != self.device or t.dim() != 1 or t.shape[0] != n or (
+                n > 1 and t.stride(0) != 1):
+            raise _invalid(f"{name}: {t.dtype} {tuple(t.shape)} on {t.device}; {n} contiguous int32 are wanted")
+        return t.data_ptr()
+
+    def _track(self, t, name: str, dtype, batch: int, ld=None):
+        """A contiguous [batch][kv_heads][track_ld] array (None stays None); its pointer and track_ld."""
+        if t is None:
+            return None, ld or 0
+        if t.dtype != dtype or t.device != self.device or t.dim() != 3 or not t.is_contiguous() or t.shape[:2] != (
+                batch, self.kv_heads):
+            raise _invalid(f"{name}: {t.dtype} {tuple(t.shape)} on {t.device}; contiguous {dtype} [{batch}]"
+                           f"[{self.kv_heads}][slots] is wanted")
+        if ld and ld != t.shape[2]:
+            raise _invalid(f"{name}: {t.shape[2]} slots where the others have {ld}")
+        return t.data_ptr(), t.shape[2]
+
+    def _scratch(self, t):
+        if t.device != self.device or not t.is_contiguous():
+            raise _invalid(f"scratch on {t.device}: contiguous memory on {self.device} is wanted")
+        return t.data_ptr(), t.numel() * t.element_size()
+
+    # ---- calls -----------------------------------------------------------------------------
+    def scratch(self, batch: int, heads: int, track_ld: int = 0):
+        """Zeroed scratch of attention / rope_attention calls of up to these
+        sizes (track_ld: that of the mass array, 0 without one); one call at a
+        time may use it."""
+        import torch
+        n = self.lib.kq_kv_attention_scratch(self.handle, batch, heads, track_ld)
+        if n == 0:
+            raise _invalid(f"attention of {batch} sequences, {heads} query heads over {self.kv_heads}")
+        return torch.zeros(n, dtype=torch.uint8, device=self.device)
+
+    def evict_scratch(self, batch: int, track_ld: int):
+        """Scratch of evict calls of these sizes; one call at a time may use it."""
+        import torch
+        n = self.lib.kq_kv_evict_scratch(self.handle, batch, track_ld)
+        if n == 0:
+            raise _invalid(f"eviction from {batch} sequences of {track_ld} tracked slots")
+        return torch.empty(n, dtype=torch.uint8, device=self.device)
+
+    def append(self, qkv, table, slots, *, theta: float, seqs=None, pos=None, q_out=None, slot_pos=None) -> None:
+        """Row r of qkv [rows][(heads + 2 kv_heads) head_dim] (q | k | v) into
+        slot slots[r] (-1: none) of sequence seqs[r] (default r), turned to
+        position pos[r] (default: the slot); the turned q into q_out."""
+        f32, i32 = self._types
+        ld = self._rows(qkv, "qkv", f32)
+        rows, batch = qkv.shape[0], table.shape[0]
+        heads = qkv.shape[1] // self.head_dim - 2 * self.kv_heads
+        if (heads + 2 * self.kv_heads) * self.head_dim != qkv.shape[1]:
+            raise _invalid(f"qkv: rows of {qkv.shape[1]} are not whole heads of {self.head_dim}")
+        q_ld = 0
+        if q_out is not None:
+            q_ld = self._rows(q_out, "q_out", f32, rows)
+            if q_out.shape[1] < heads * self.head_dim:
+                raise _invalid(f"q_out: rows of {q_out.shape[1]} for {heads} heads of {self.head_dim}")
+        sp, track = self._track(slot_pos, "slot_pos", i32, batch)
+        self.ctx.check(self.lib.kq_kv_append(
+            self.handle, qkv.data_ptr(), ld, rows, heads, self._vector(seqs, "seqs", rows),
+            self._vector(slots, "slots", rows), self._vector(pos, "pos", rows), table.data_ptr(),
+            self._rows(table, "table", i32), batch, theta, q_out.data_ptr() if q_out is not None else None, q_ld, sp,
+            track), "kq_kv_append")
+
+    def attention(self, q, table, lens, out, scratch, mass=None) -> None:
+        """out[b] = attention of q[b] [heads][head_dim] (turned already) over
+        slots [0, lens[b]) of sequence b (0: zeros); mass accumulates each
+        slot's weight, summed over the query heads of its kv head."""
+        f32, i32 = self._types
+        batch, cols = q.shape
+        heads = cols // self.head_dim
+        q_ld, out_ld = self._rows(q, "q", f32), self._rows(out, "out", f32, batch)
+        if heads * self.head_dim != cols or out.shape[1] < cols:
+            raise _invalid(f"q rows of {cols} and out rows of {out.shape[1]} for heads of {self.head_dim}")
+        m, track = self._track(mass, "mass", f32, batch)
+        sp, sb = self._scratch(scratch)
+        self.ctx.check(self.lib.kq_kv_attention(
+            self.handle, q.data_ptr(), q_ld, out.data_ptr(), out_ld, batch, heads, table.data_ptr(),
+            self._rows(table, "table", i32, batch), self._vector(lens, "lens", batch), m, track, sp, sb),
+            "kq_kv_attention")
+
+    def rope_attention(self, qkv, table, lens, out, scratch, *, theta: float, pos=None, mass=None,
+                       slot_pos=None) -> None:
+        """The same for the step's new tokens: q and k of qkv[b] (q | k | v)
+        turned to pos[b] (default lens[b] - 1), k and v appended at slot
+        lens[b] - 1, then the attention; the new slot's mass starts anew and its
+        position goes to slot_pos."""
+        f32, i32 = self._types
+        batch, cols = qkv.shape
+        heads = cols // self.head_dim - 2 * self.kv_heads
+        ld, out_ld = self._rows(qkv, "qkv", f32), self._rows(out, "out", f32, batch)
+        if (heads + 2 * self.kv_heads) * self.head_dim != cols or out.shape[1] < heads * self.head_dim:
+            raise _invalid(f"qkv rows of {cols} and out rows of {out.shape[1]} for heads of {self.head_dim}")
+        m, track = self._track(mass, "mass", f32, batch)
+        p, track = self._track(slot_pos, "slot_pos", i32, batch, track)
+        sp, sb = self._scratch(scratch)
+        self.ctx.check(self.lib.kq_kv_rope_attention(
+            self.handle, qkv.data_ptr(), ld, out.data_ptr(), out_ld, batch, heads, table.data_ptr(),
+            self._rows(table, "table", i32, batch), self._vector(lens, "lens", batch),
+            self._vector(pos, "pos", batch), theta, m, p, track, sp, sb), "kq_kv_rope_attention")
+
+    def evict(self, table, lens, lens_out, mass, slot_pos, mass_out, pos_out, keep: int, scratch,
+              recent_from=None) -> None:
+        """Cut sequences of more than `keep` slots to `keep`: the slots at
+        positions >= recent_from[b], then those of the greatest mass.  The
+        outputs may be the inputs."""
+        f32, i32 = self._types
+        batch = table.shape[0]
+        m, track = self._track(mass, "mass", f32, batch)
+        p, _ = self._track(slot_pos, "slot_pos", i32, batch, track)
+        mo, _ = self._track(mass_out, "mass_out", f32, batch, track)
+        po, _ = self._track(pos_out, "pos_out", i32, batch, track)
+        sp, sb = self._scratch(scratch)
+        self.ctx.check(self.lib.kq_kv_evict(
+            self.handle, batch, table.data_ptr(), self._rows(table, "table", i32), self._vector(lens, "lens", batch),
+            self._vector(lens_out, "lens_out", batch), m, p, mo, po, track,
+            self._vector(recent_from, "recent_from", batch), keep, sp, sb), "kq_kv_evict")
+
+    def close(self) -> None:
+        if getattr(self, "handle", None):
+            self.lib.kq_kv_destroy(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
