@@ -87,6 +87,7 @@ struct kq_weight {
 struct kq_kv {
   kq_ctx* ctx = nullptr;
   kq::KvPool pool;
+  kq::KvMaps maps;
 };
 
 // A decode-step program (kq_step_*): its stages on the host, and once built,
@@ -1302,6 +1303,10 @@ int kq_kv_create(kq_ctx* ctx, void* k_pool, void* v_pool, int64_t pages, int64_t
   kv->pool.page_size = page_size;
   kv->pool.hkv = kv_heads;
   kv->pool.hd = head_dim;
+  if (!kq::kv_make_maps(kv->pool, &kv->maps)) {
+    delete kv;
+    return fail(ctx, KQ_ERR_CUDA, "kq_kv_create: the driver refused the pools' TMA descriptors");
+  }
   *out = kv;
   return KQ_OK;
 }
@@ -1399,6 +1404,7 @@ static int kv_attention_impl(kq_kv* kv, const char* what, bool rope, const float
     return fail(ctx, KQ_ERR_SHORT_BUFFER, "%s: scratch of %zu bytes is too small", what, scratch_bytes);
   kq::KvAttnArgs a;
   a.pool = kv->pool;
+  a.rope = rope;
   a.q = q;
   a.q_ld = q_ld;
   a.out = out;
@@ -1419,7 +1425,7 @@ static int kv_attention_impl(kq_kv* kv, const char* what, bool rope, const float
   DeviceGuard g(ctx->device);
   if (g.status != cudaSuccess) return cuda_fail(ctx, g.status, "cudaSetDevice");
   int launches = 0;
-  const cudaError_t e = kq::kv_attention(a, rope, &launches, ctx->stream);
+  const cudaError_t e = kq::kv_attention(a, kv->maps, &launches, ctx->stream);
   ctx->launches += launches;
   return dec_status(ctx, e, what);
 }

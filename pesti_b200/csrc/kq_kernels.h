@@ -6,6 +6,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
+
 namespace kq {
 
 constexpr int QK = 256;         // weights per K-quant superblock
@@ -357,6 +359,13 @@ struct KvPool {
   int64_t pages = 0, page_ld = 0;
   int page_size = 0, hkv = 0, hd = 0;
 };
+// TMA descriptors of the two pools: boxes of kv_box_rows slots of one page and head.
+struct KvMaps {
+  CUtensorMap k, v;
+};
+// The largest power of two that divides the page and is at most one tile (64 slots).
+inline int kv_box_rows(int page_size) { return std::min(64, page_size & -page_size); }
+bool kv_make_maps(const KvPool& pool, KvMaps* maps);
 // Per-device set-up of the paged-cache kernels (shared-memory sizes).
 cudaError_t kv_init_device();
 struct KvAppendArgs {
@@ -379,6 +388,7 @@ struct KvAppendArgs {
 cudaError_t kv_append(const KvAppendArgs& a, cudaStream_t s);
 struct KvAttnArgs {
   KvPool pool;
+  bool rope;
   const float* q;  // token b's query heads at q + b * q_ld (rope: the fused qkv row)
   int64_t q_ld;
   float* out;
@@ -399,7 +409,7 @@ struct KvAttnArgs {
 // head_dim 64, 128 or 256, 1 to KV_MAX_GROUP query heads per kv head.
 constexpr int KV_MAX_GROUP = 16;
 size_t kv_attention_scratch_bytes(int64_t batch, int hq, int hkv, int hd, int64_t track_len, int num_sms);
-cudaError_t kv_attention(const KvAttnArgs& a, bool rope, int* launches, cudaStream_t s);
+cudaError_t kv_attention(const KvAttnArgs& a, const KvMaps& maps, int* launches, cudaStream_t s);
 struct KvEvictArgs {
   KvPool pool;
   int64_t batch;
@@ -439,6 +449,10 @@ struct SampleArgs {
 cudaError_t dec_sample(const SampleArgs& a, cudaStream_t s);
 
 // ---- tensor-core (tcgen05) path: kq_mma.cu ----
+// A tiled TMA descriptor of `rank` (at most 5) dimensions, innermost first,
+// element strides 1; false where the driver refuses it.
+bool encode_tiled_map(CUtensorMap* map, CUtensorMapDataType dt, int rank, const void* base, const cuuint64_t* dims,
+                      const cuuint64_t* strides, const cuuint32_t* box, CUtensorMapSwizzle swz);
 // Build the TMA descriptors of a GGUF weight (after its device arrays exist).
 bool tc_make_weight_maps(DevWeight& w);
 // Per-device set-up of the tcgen05 kernels (shared-memory carve-outs).

@@ -1,9 +1,7 @@
-// kq_paged.cu -- a paged f16 key-value cache: appending rows, attention of one
-// new token per sequence, and eviction by accumulated attention weight
-// (include/pesti_decoder.h, kq_kv_*).
-#include "kq_common.cuh"
+// kq_paged.cu -- a paged f16 key-value cache: appending rows and eviction by
+// accumulated attention weight (include/pesti_decoder.h, kq_kv_append and
+// kq_kv_evict).
 #include "kq_paged.cuh"
-#include "kq_sm100.cuh"
 
 #include <cuda_fp16.h>
 #include <math.h>
@@ -13,26 +11,11 @@
 namespace kq {
 namespace {
 
-__device__ __forceinline__ void pdl_enter() {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-}
-
-__device__ __forceinline__ void kv_error(int* err, int code) { atomicCAS(err, 0, code); }
-
-// cos / sin of pos * theta^(-i / half).  The angle is reduced in 64 bits: at
-// position 100,000 an f32 angle is off by 4e-3, where the f32 result of this
-// form stays within 1e-7 of the exact one.
-__device__ __forceinline__ void rope_turn(int32_t pos, int i, int half, double log2_theta, float& c, float& s) {
-  const double t = (double)pos * exp2(-(double)i / (double)half * log2_theta) * 0.15915494309189533577;
-  sincospif(2.f * (float)(t - rint(t)), &s, &c);
-}
-
 // ---- append ---------------------------------------------------------------------
 // One CTA per row, one thread per (head, pair): q and k turned, k and v rounded
 // to f16 into their slot.
 __global__ void __launch_bounds__(256) kv_append_kernel(const KvAppendArgs A) {
-  pdl_enter();
+  kv_pdl_enter();
   const int half = A.pool.hd / 2, hkv = A.pool.hkv;
   const int64_t r = blockIdx.x;
   const int32_t slot = A.slots[r];
@@ -71,129 +54,6 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const KvAppendArgs A) {
   }
   if (A.slot_pos)
     for (int h = threadIdx.x; h < hkv; h += blockDim.x) A.slot_pos[(b * hkv + h) * A.track_ld + slot] = pos;
-}
-
-// ---- attention ------------------------------------------------------------------
-// One CTA per (kv head, sequence): tiles of 32 slots, a thread per score, the
-// running maximum and sum of the softmax per query head.
-constexpr int AP_TILE = 32, AP_THREADS = 256, AP_MAX_HD = 256;
-
-template <bool ROPE>
-__global__ void __launch_bounds__(AP_THREADS) kv_attn_kernel(const KvAttnArgs A) {
-  pdl_enter();
-  __shared__ float q[KV_MAX_GROUP * AP_MAX_HD], acc[KV_MAX_GROUP * AP_MAX_HD];
-  __shared__ float sc[KV_MAX_GROUP * AP_TILE], mx[KV_MAX_GROUP], sum[KV_MAX_GROUP], corr[KV_MAX_GROUP];
-  const int hk = blockIdx.x, hd = A.pool.hd, half = hd / 2, hkv = A.pool.hkv, G = A.hq / hkv;
-  const int64_t b = blockIdx.y;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  int64_t most = A.table_ld * A.pool.page_size;
-  if (A.mass || A.slot_pos) most = min(most, A.track_ld);
-  bool bad;
-  const int64_t len = kv_len(A.lens[b], most, &bad);
-  if (bad && tid == 0) kv_error(A.err, KV_ERR_LEN);
-  float* out = A.out + b * A.out_ld + (int64_t)hk * G * hd;
-  if (len == 0) {
-    for (int e = tid; e < G * hd; e += AP_THREADS) out[e] = 0.f;
-    return;
-  }
-  const __half* kc = static_cast<const __half*>(A.pool.k);
-  const __half* vc = static_cast<const __half*>(A.pool.v);
-  const int32_t* table = A.table + b * A.table_ld;
-  const float* row = A.q + b * A.q_ld;
-  const float scale = 1.f / sqrtf((float)hd);
-  const int32_t pos = ROPE ? (A.pos ? A.pos[b] : (int32_t)(len - 1)) : 0;
-  for (int e = tid; e < G * half; e += AP_THREADS) {
-    const int g = e / half, i = e - g * half;
-    const float* p = row + (int64_t)(hk * G + g) * hd;
-    float x = p[i], y = p[i + half];
-    if (ROPE) {
-      float c, s;
-      rope_turn(pos, i, half, A.log2_theta, c, s);
-      const float t = x * c - y * s;
-      y = x * s + y * c;
-      x = t;
-    }
-    q[g * hd + i] = x * scale;
-    q[g * hd + i + half] = y * scale;
-  }
-  for (int e = tid; e < G * hd; e += AP_THREADS) acc[e] = 0.f;
-  if (tid < G) mx[tid] = -INFINITY, sum[tid] = 0.f;
-  if (ROPE) {
-    const int64_t o = kv_row(A.pool, table[(len - 1) / A.pool.page_size], len - 1, hk);
-    const float* kp = row + (int64_t)(A.hq + hk) * hd;
-    const float* vp = kp + (int64_t)hkv * hd;
-    for (int i = tid; i < half && o >= 0; i += AP_THREADS) {
-      float c, s;
-      rope_turn(pos, i, half, A.log2_theta, c, s);
-      __half* kw = static_cast<__half*>(A.pool.k) + o;
-      __half* vw = static_cast<__half*>(A.pool.v) + o;
-      kw[i] = __float2half_rn(kp[i] * c - kp[i + half] * s);
-      kw[i + half] = __float2half_rn(kp[i] * s + kp[i + half] * c);
-      vw[i] = __float2half_rn(vp[i]);
-      vw[i + half] = __float2half_rn(vp[i + half]);
-    }
-    if (tid == 0 && A.slot_pos) A.slot_pos[(b * hkv + hk) * A.track_ld + len - 1] = pos;
-  }
-  __syncthreads();
-  auto scores = [&](int64_t t0, int n) {
-    for (int e = tid; e < G * AP_TILE; e += AP_THREADS) {
-      const int g = e / AP_TILE, j = e - g * AP_TILE;
-      float v = -INFINITY;
-      if (j < n) {
-        const int64_t o = kv_row(A.pool, table[(t0 + j) / A.pool.page_size], t0 + j, hk);
-        if (o < 0) kv_error(A.err, KV_ERR_PAGE);
-        v = 0.f;
-        for (int d = 0; d < hd && o >= 0; ++d) v = fmaf(q[g * hd + d], __half2float(kc[o + d]), v);
-      }
-      sc[e] = v;
-    }
-  };
-  for (int64_t t0 = 0; t0 < len; t0 += AP_TILE) {
-    const int n = (int)min((int64_t)AP_TILE, len - t0);
-    scores(t0, n);
-    __syncthreads();
-    for (int g = warp; g < G; g += AP_THREADS / 32) {
-      const float v = sc[g * AP_TILE + lane];
-      float m = v;
-      for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-      const float mnew = fmaxf(mx[g], m);
-      const float p = lane < n ? __expf(v - mnew) : 0.f;
-      float ps = p;
-      for (int o = 16; o > 0; o >>= 1) ps += __shfl_xor_sync(0xffffffffu, ps, o);
-      sc[g * AP_TILE + lane] = p;
-      __syncwarp();
-      if (lane == 0) {
-        corr[g] = __expf(mx[g] - mnew);
-        sum[g] = sum[g] * corr[g] + ps;
-        mx[g] = mnew;
-      }
-    }
-    __syncthreads();
-    for (int e = tid; e < G * hd; e += AP_THREADS) {
-      const int g = e / hd, d = e - g * hd;
-      float v = acc[e] * corr[g];
-      for (int j = 0; j < n; ++j) {
-        const int64_t o = kv_row(A.pool, table[(t0 + j) / A.pool.page_size], t0 + j, hk);
-        if (o >= 0) v = fmaf(sc[g * AP_TILE + j], __half2float(vc[o + d]), v);
-      }
-      acc[e] = v;
-    }
-    __syncthreads();
-  }
-  for (int e = tid; e < G * hd; e += AP_THREADS) out[e] = acc[e] / sum[e / hd];
-  if (!A.mass) return;
-  float* mass = A.mass + (b * hkv + hk) * A.track_ld;
-  for (int64_t t0 = 0; t0 < len; t0 += AP_TILE) {
-    const int n = (int)min((int64_t)AP_TILE, len - t0);
-    scores(t0, n);
-    __syncthreads();
-    if (tid < n) {
-      float v = 0.f;
-      for (int g = 0; g < G; ++g) v += __expf(sc[g * AP_TILE + tid] - mx[g]) / sum[g];
-      mass[t0 + tid] = ROPE && t0 + tid == len - 1 ? v : mass[t0 + tid] + v;
-    }
-    __syncthreads();
-  }
 }
 
 // ---- eviction ---------------------------------------------------------------------
@@ -241,7 +101,7 @@ struct EvictPlan {  // one (sequence, kv head)
 __host__ __device__ __forceinline__ int64_t evict_list(int64_t track_ld) { return (track_ld + 3) & ~int64_t(3); }
 
 __global__ void __launch_bounds__(EV_THREADS) kv_evict_select_kernel(const KvEvictArgs A) {
-  pdl_enter();
+  kv_pdl_enter();
   __shared__ unsigned hist[256];
   __shared__ int sums[32];
   __shared__ uint32_t pick[2];  // digit, how many of it still to keep
@@ -331,7 +191,7 @@ __global__ void __launch_bounds__(EV_THREADS) kv_evict_select_kernel(const KvEvi
 }
 
 __global__ void __launch_bounds__(256) kv_evict_move_kernel(const KvEvictArgs A) {
-  pdl_enter();
+  kv_pdl_enter();
   const int hk = blockIdx.y, hkv = A.pool.hkv;
   const int64_t b = blockIdx.z, bh = b * hkv + hk;
   const EvictPlan plan = static_cast<const EvictPlan*>(A.scratch)[bh];
@@ -362,19 +222,8 @@ __global__ void __launch_bounds__(256) kv_evict_move_kernel(const KvEvictArgs A)
 
 }  // namespace
 
-cudaError_t kv_init_device() { return cudaSuccess; }
-
 cudaError_t kv_append(const KvAppendArgs& a, cudaStream_t s) {
   return launch_pdl(kv_append_kernel, dim3((unsigned)a.rows), dim3(256), 0, s, a);
-}
-
-size_t kv_attention_scratch_bytes(int64_t, int, int, int, int64_t, int) { return 256; }
-
-cudaError_t kv_attention(const KvAttnArgs& a, bool rope, int* launches, cudaStream_t s) {
-  dim3 grid((unsigned)a.pool.hkv, (unsigned)a.batch);
-  *launches = 1;
-  return rope ? launch_pdl(kv_attn_kernel<true>, grid, dim3(AP_THREADS), 0, s, a)
-              : launch_pdl(kv_attn_kernel<false>, grid, dim3(AP_THREADS), 0, s, a);
 }
 
 size_t kv_evict_scratch_bytes(int64_t batch, int hkv, int64_t track_ld) {

@@ -25,4 +25,21 @@ __host__ __device__ __forceinline__ int64_t kv_row(const KvPool& p, int32_t page
   return (int64_t)page * p.page_ld + ((int64_t)head * p.page_size + slot % p.page_size) * p.hd;
 }
 
+#ifdef __CUDACC__
+__device__ __forceinline__ void kv_pdl_enter() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+__device__ __forceinline__ void kv_error(int* err, int code) { atomicCAS(err, 0, code); }
+
+// cos / sin of pos * theta^(-i / half).  The angle is reduced in 64 bits: at
+// position 100,000 an f32 angle is off by 4e-3, where the f32 result of this
+// form stays within 1e-7 of the exact one.
+__device__ __forceinline__ void rope_turn(int32_t pos, int i, int half, double log2_theta, float& c, float& s) {
+  const double t = (double)pos * exp2(-(double)i / (double)half * log2_theta) * 0.15915494309189533577;
+  sincospif(2.f * (float)(t - rint(t)), &s, &c);
+}
+#endif
+
 }  // namespace kq
