@@ -41,6 +41,7 @@ using sm100::smem_u32;
 
 constexpr int PA_TILE = 64;     // slots per ring stage
 constexpr int PA_SHIFT = 14;    // P carries 2^14
+constexpr int PA_PARTS = 512;   // CTAs that can share a pair: two per SM
 constexpr int PA_SET = 128;     // threads of the four warps that share a set of eight query heads
 
 template <int HD, int NS>
@@ -49,8 +50,8 @@ struct PaCfg {
   static constexpr int CW = 4 * NS, THREADS = (CW + 1) * 32;
   static constexpr int TILE_B = PA_TILE * HD * 2, STAGE = 2 * TILE_B;
   // two CTAs per SM where 96 KB of ring each still leaves room for two
-  static constexpr int CTAS = HD == 64 || (HD == 128 && NS == 1) ? 2 : 1;
-  static constexpr int STAGES = HD == 64 ? 6 : HD == 128 ? (NS == 1 ? 3 : 6) : (NS == 1 ? 3 : 2);
+  static constexpr int CTAS = NS == 1 && HD <= 128 ? 2 : 1;
+  static constexpr int STAGES = HD == 256 ? (NS == 1 ? 3 : 2) : (NS == 1 ? 384 : 768) / HD;
   static constexpr int QF = STAGES * STAGE;            // q fragments [NS][KS][32] {hi, hi, lo, lo}
   static constexpr int RED = QF + NS * KS * 512;       // [NS][2][8][HD] f32: the warps' sums
   static constexpr int ML = RED + NS * 2 * 8 * HD * 4;  // [NS][4][8] {max, sum}
@@ -59,6 +60,7 @@ struct PaCfg {
   static constexpr int BAR = NEW + NS * 2 * HD * 2;    // full, empty
   static constexpr int LAST = BAR + 2 * STAGES * 8;    // [NS][2] flags
   static constexpr int END = LAST + NS * 8;
+  static_assert(NS * PA_PARTS * 8 * 8 <= QF, "the join's {max, sum} lie in the ring");
   static_assert(END <= 232448 && CTAS * (END + 1024) <= 233472, "shared memory");
 };
 
@@ -183,7 +185,7 @@ struct PaWalk {
         const int64_t rem = f - base - __shfl_sync(0xffffffffu, incl - n, at) * hkv;
         const int u = __shfl_sync(0xffffffffu, n, at);
         b = b0 + at;
-        hk = (int)(rem / u);
+        hk = (int)div(rem, u);
         v = (int)(rem - (int64_t)hk * u);
         nt = u - PA_PAIR;
         bool bad;
@@ -193,8 +195,12 @@ struct PaWalk {
       base += here;
     }
   }
-  __device__ __forceinline__ int64_t begin(int cta) const { return total * cta / ctas; }
-  __device__ __forceinline__ int owner(int64_t unit) const { return (int)(((unit + 1) * ctas - 1) / total); }
+  // a / b; 64-bit division is a long sequence of instructions, rarely needed
+  static __device__ __forceinline__ int64_t div(int64_t a, int64_t b) {
+    return (uint64_t)(a | b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
+  }
+  __device__ __forceinline__ int64_t begin(int cta) const { return div(total * cta, ctas); }
+  __device__ __forceinline__ int owner(int64_t unit) const { return (int)div((unit + 1) * ctas - 1, total); }
   __device__ __forceinline__ int here() const { return (int)min((int64_t)(nt + PA_PAIR - v), f1 - f); }
   __device__ __forceinline__ int j0() const { return max(0, v - PA_PAIR); }        // this CTA's tiles of the pair:
   __device__ __forceinline__ int j1() const { return max(0, v + here() - PA_PAIR); }  // [j0, j1), j1 <= nt
@@ -657,55 +663,92 @@ __global__ void __launch_bounds__(PaCfg<HD, NS>::THREADS, PaCfg<HD, NS>::CTAS)
   if (!pends) return;
 
   // ---- shared pairs: the last CTA to arrive joins the parts in slot order ----
+  if (NS > 1) asm volatile("bar.sync 3, %0;" ::"n"(C::CW * 32) : "memory");  // the ring is used up by every set
   if (w == 0) {
-    __threadfence();
     __syncwarp();
     if (lane < pends) {
+      __threadfence();  // the warp's parts before the arrival, and what the arrival found before the join
       unsigned* cnt = ctr + 2 * (lane ? pend_c0[1] : pend_c0[0]) + set;
       const int others = lane ? pend_c1[1] - pend_c0[1] : pend_c1[0] - pend_c0[0];
       const bool last = atomicAdd(cnt, 1u) == (unsigned)others;
-      if (last) *cnt = 0u;  // ready for the next call (stream-ordered)
+      if (last) {
+        __threadfence();
+        *cnt = 0u;  // ready for the next call (stream-ordered)
+      }
       last_s[lane] = last;
     }
   }
   bar_set(set);
   for (int k = 0; k < pends; ++k) {
     if (!last_s[k]) continue;
-    __threadfence();
-    const int c0 = k ? pend_c0[1] : pend_c0[0], parts = (k ? pend_c1[1] : pend_c1[0]) - c0;  // besides the first
+    const int c0 = k ? pend_c0[1] : pend_c0[0], parts = (k ? pend_c1[1] : pend_c1[0]) - c0 + 1;
     const int64_t out_row = k ? pend_row[1] : pend_row[0];
     const int head0 = k ? pend_head[1] : pend_head[0];
-    const int64_t step = 2 * NS * 8;
-    for (int e = stid; e < nh * (HD / 4); e += PA_SET) {
-      const int h = e / (HD / 4), d4 = e - h * (HD / 4);
-      const int64_t at0 = ((2 * (int64_t)c0 + 1) * NS + set) * 8 + h;  // the pair's first part
-      const int64_t at1 = (2 * (int64_t)(c0 + 1) * NS + set) * 8 + h;  // its others, one CTA apart
-      float2 ml = __ldcg(part_ml + at0);
-      float4 v = __ldcg(reinterpret_cast<const float4*>(part + at0 * HD) + d4);
-      float M = ml.x;
-#pragma unroll 8
-      for (int p = 0; p < parts; ++p) M = fmaxf(M, __ldcg(part_ml + at1 + p * step).x);
-      float f = ex2(ml.x - M), L = f * ml.y;
-      float4 r = make_float4(f * v.x, f * v.y, f * v.z, f * v.w);
-#pragma unroll 8
-      for (int p = 0; p < parts; ++p) {
-        ml = __ldcg(part_ml + at1 + p * step);
-        v = __ldcg(reinterpret_cast<const float4*>(part + (at1 + p * step) * HD) + d4);
-        f = ex2(ml.x - M);
-        L = fmaf(f, ml.y, L);
-        r.x = fmaf(f, v.x, r.x);
-        r.y = fmaf(f, v.y, r.y);
-        r.z = fmaf(f, v.z, r.z);
-        r.w = fmaf(f, v.w, r.w);
+    // part p's place: the pair begins in c0's second slot and goes on in the others' first
+    auto place = [&](int p) { return ((2 * (int64_t)(c0 + p) + (p == 0)) * NS + set) * 8; };
+    // every part's {max, sum} into the ring (its copies are used up); while they
+    // come, the first sums: a thread takes a float4 column of parts pg, pg + np, ...
+    const int cols = nh * (HD / 4), np = max(1, PA_SET / cols);
+    float2* ml_p = reinterpret_cast<float2*>(sm) + set * PA_PARTS * 8;
+    for (int e = stid; e < parts * nh; e += PA_SET) ml_p[e] = __ldcg(part_ml + place(e / nh) + e % nh);
+    constexpr int AHEAD = 16;
+    for (int e = stid; e < (np > 1 ? PA_SET : (cols + PA_SET - 1) / PA_SET * PA_SET); e += PA_SET) {
+      const int pg = np > 1 ? e / cols : 0, col = np > 1 ? e - pg * cols : e;
+      const bool mine = pg < np && col < cols;
+      const int h = mine ? col / (HD / 4) : 0, d4 = col - h * (HD / 4);
+      auto sum_of = [&](int p) {
+        return mine && p < parts ? __ldcg(reinterpret_cast<const float4*>(part + (place(p) + h) * HD) + d4)
+                                 : make_float4(0.f, 0.f, 0.f, 0.f);
+      };
+      float4 v[AHEAD];
+#pragma unroll
+      for (int q = 0; q < AHEAD; ++q) v[q] = sum_of(pg + q * np);
+      bar_set(set);
+      float M = -INFINITY, L = 0.f;
+      for (int p = 0; p < parts; ++p) M = fmaxf(M, ml_p[p * nh + h].x);
+      float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int p0 = pg; p0 < parts; p0 += AHEAD * np) {
+#pragma unroll
+        for (int q = 0; q < AHEAD; ++q) {
+          const int p = p0 + q * np;
+          const float2 ml = p < parts ? ml_p[p * nh + h] : make_float2(-INFINITY, 0.f);
+          const float f = ex2(ml.x - M);
+          L = fmaf(f, ml.y, L);
+          r.x = fmaf(f, v[q].x, r.x);
+          r.y = fmaf(f, v[q].y, r.y);
+          r.z = fmaf(f, v[q].z, r.z);
+          r.w = fmaf(f, v[q].w, r.w);
+          v[q] = sum_of(p + AHEAD * np);
+        }
       }
-      const float inv = 1.f / L;
-      float* out = A.out + out_row + h * HD + 4 * d4;
-      out[0] = r.x * inv;
-      out[1] = r.y * inv;
-      out[2] = r.z * inv;
-      out[3] = r.w * inv;
-      if (A.mass && d4 == 0) stats[head0 + h] = make_float2(M, L);
+      if (np > 1) {  // the parts' groups, in order
+        float4* rs = reinterpret_cast<float4*>(red);
+        rs[stid] = r;
+        float* ls = red + PA_SET * 4;
+        ls[stid] = L;
+        bar_set(set);
+        if (pg == 0) {
+          for (int q = 1; q < np; ++q) {
+            const float4 x = rs[q * cols + col];
+            r.x += x.x;
+            r.y += x.y;
+            r.z += x.z;
+            r.w += x.w;
+            L += ls[q * cols + col];
+          }
+        }
+      }
+      if (mine && pg == 0) {
+        const float inv = 1.f / L;
+        float* out = A.out + out_row + h * HD + 4 * d4;
+        out[0] = r.x * inv;
+        out[1] = r.y * inv;
+        out[2] = r.z * inv;
+        out[3] = r.w * inv;
+        if (A.mass && d4 == 0) stats[head0 + h] = make_float2(M, L);
+      }
     }
+    bar_set(set);  // ml_p and red are free again
   }
 }
 
@@ -737,7 +780,7 @@ cudaError_t launch_attn(const PaParams& P, const KvMaps& maps, int num_sms, cuda
   using C = PaCfg<HD, NS>;
   const KvAttnArgs& a = P.a;
   const int64_t tiles = a.batch * a.pool.hkv * ((a.table_ld * a.pool.page_size + PA_TILE - 1) / PA_TILE);
-  const unsigned grid = (unsigned)std::min<int64_t>((int64_t)C::CTAS * num_sms, tiles);
+  const unsigned grid = (unsigned)std::min<int64_t>(std::min<int64_t>(C::CTAS * num_sms, PA_PARTS), tiles);
   return launch_pdl(kv_attn_kernel<HD, NS>, dim3(grid), dim3(C::THREADS), C::END, s, maps.k, maps.v, P);
 }
 
