@@ -327,6 +327,7 @@ int kq_ctx_create(int device, kq_ctx** out) {
   if (e == cudaSuccess) e = kq::imma_init_device();
   if (e == cudaSuccess) e = kq::dec_init_device();
   if (e == cudaSuccess) e = kq::kv_init_device();
+  if (e == cudaSuccess) e = kq::kv_evict_init_device();
   if (e == cudaSuccess) e = kq::sample_init_device();
   if (e == cudaSuccess) e = kq::kx_init_device();
   if (e == cudaSuccess) e = kq::step_init_device();
@@ -1514,7 +1515,7 @@ int kq_dec_sample(kq_ctx* ctx, const float* logits, int64_t ld, int64_t batch, i
   a.kept = kept;
   DeviceGuard g(ctx->device);
   if (g.status != cudaSuccess) return cuda_fail(ctx, g.status, "cudaSetDevice");
-  const cudaError_t e = kq::dec_sample(a, ctx->stream);
+  const cudaError_t e = kq::dec_sample(a, ctx->num_sms, ctx->stream);
   ctx->launches += e == cudaSuccess;
   return dec_status(ctx, e, "kq_dec_sample");
 }

@@ -368,6 +368,7 @@ inline int kv_box_rows(int page_size) { return std::min(64, page_size & -page_si
 bool kv_make_maps(const KvPool& pool, KvMaps* maps);
 // Per-device set-up of the paged-cache kernels (shared-memory sizes).
 cudaError_t kv_init_device();
+cudaError_t kv_evict_init_device();
 struct KvAppendArgs {
   KvPool pool;
   const float* qkv;  // row r at qkv + r * ld: q (hq heads) | k (hkv) | v (hkv)
@@ -446,7 +447,7 @@ struct SampleArgs {
   float* prob;    // or NULL
   int32_t* kept;  // or NULL
 };
-cudaError_t dec_sample(const SampleArgs& a, cudaStream_t s);
+cudaError_t dec_sample(const SampleArgs& a, int num_sms, cudaStream_t s);
 
 // ---- tensor-core (tcgen05) path: kq_mma.cu ----
 // A tiled TMA descriptor of `rank` (at most 5) dimensions, innermost first,
