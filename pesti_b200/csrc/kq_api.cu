@@ -1343,7 +1343,7 @@ int kq_kv_append(kq_kv* kv, const float* qkv, int64_t ld, int64_t rows, int head
   if (!kv) return KQ_ERR_INVALID_ARG;
   kq_ctx* ctx = kv->ctx;
   const char* what = "kq_kv_append";
-  if (!qkv || !slots) return fail(ctx, KQ_ERR_INVALID_ARG, "%s: null qkv or slots", what);
+  if (rows > 0 && (!qkv || !slots)) return fail(ctx, KQ_ERR_INVALID_ARG, "%s: null qkv or slots", what);
   if (int rc = kv_check(kv, what, table, table_ld, batch)) return rc;
   if (int rc = kv_heads_check(kv, what, heads)) return rc;
   const int64_t hd = kv->pool.hd;

@@ -44,14 +44,14 @@ class PagedCache:
 
     def __init__(self, ctx: "kq.Context", k, v):
         import torch
-        if k.dim() != 4 or k.shape != v.shape or k.stride() != v.stride():
+        if k.dim() != 4 or 0 in k.shape or k.shape != v.shape or k.stride() != v.stride():
             raise _invalid(f"pools of shapes {tuple(k.shape)} and {tuple(v.shape)}: one shape and stride is wanted")
         if k.dtype != torch.float16 or v.dtype != torch.float16:
             raise _invalid(f"pools of {k.dtype} and {v.dtype}: float16 is wanted")
         self.pages, self.kv_heads, self.page_size, self.head_dim = k.shape
-        inner = (self.page_size * self.head_dim, self.head_dim, 1)
-        if k.stride()[1:] != inner:
+        if not k[0].is_contiguous():
             raise _invalid(f"pool strides {k.stride()}: the pages must be contiguous")
+        page_ld = k.stride(0) if self.pages > 1 else k[0].numel()
         self.device = torch.device("cuda", ctx.device)
         if k.device != self.device or v.device != self.device:
             raise _invalid(f"pools on {k.device} and {v.device}, context on {self.device}")
@@ -59,7 +59,7 @@ class PagedCache:
         self.lib = _bind(ctx.lib)
         self._types = torch.float32, torch.int32
         h = ctypes.c_void_p()
-        ctx.check(self.lib.kq_kv_create(ctx.handle, k.data_ptr(), v.data_ptr(), self.pages, k.stride(0),
+        ctx.check(self.lib.kq_kv_create(ctx.handle, k.data_ptr(), v.data_ptr(), self.pages, page_ld,
                                         self.page_size, self.kv_heads, self.head_dim, ctypes.byref(h)), "kq_kv_create")
         self.handle = h
 
