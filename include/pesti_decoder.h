@@ -256,7 +256,8 @@ int kq_dec_sample(kq_ctx *ctx, const float *logits, int64_t ld, int64_t batch, i
                   const int32_t *top_k, const float *top_p, const float *min_p, const float *u, int32_t *tokens,
                   float *prob, int32_t *kept);
 
-/* out[b] = table[tokens[b]] (Model::embed, model.rs:966-984); table f32 [vocab][dim]. */
+/* out[b] = table[tokens[b]] (Model::embed, model.rs:966-984); table f32 [vocab][dim].
+ * A negative token (kq_dec_sample's -1) gives a row of zeros. */
 int kq_dec_embed(kq_ctx *ctx, const float *table, const int32_t *tokens, float *out, int64_t out_ld,
                  int64_t batch, int64_t dim);
 

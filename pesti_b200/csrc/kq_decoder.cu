@@ -517,7 +517,7 @@ __global__ void embed_kernel(const float* __restrict__ table, const int* __restr
   pdl_enter();
   const int64_t tok = tokens[blockIdx.y];
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < dim; i += (int64_t)gridDim.x * blockDim.x)
-    out[(int64_t)blockIdx.y * out_ld + i] = table[tok * dim + i];
+    out[(int64_t)blockIdx.y * out_ld + i] = tok < 0 ? 0.f : table[tok * dim + i];  // -1: a row without a token
 }
 
 template <int HD, int G>

@@ -34,7 +34,7 @@ import zlib
 from dataclasses import dataclass
 from typing import Optional
 
-from . import kq
+from . import kq, paged, sampling
 
 SWIGLU_REFERENCE = 0  # pesti's swiglu (layer.rs:16-29): negative gates use g / (1 + e^g)
 SWIGLU_SILU = 1
@@ -154,8 +154,13 @@ class Decoder:
     def __init__(self, cfg: DecoderConfig, ctx: "kq.Context", batch: int, context_len: int, max_new: int = 8,
                  world: int = 1, rank: int = 0, tp: Optional["kq.TensorParallel"] = None, seed: int = 0,
                  swiglu_mode: int = SWIGLU_REFERENCE, kv_scale: float = 1.0, keep_raw: bool = False,
-                 fused: bool = True, prefetch: bool = False, step_kernel: bool = False):
+                 fused: bool = True, prefetch: bool = False, step_kernel: bool = False, page_size: int = 0,
+                 track: bool = False):
         import torch
+        if page_size and step_kernel:
+            raise ValueError("the persistent step kernel reads a contiguous cache")
+        if track and not page_size:
+            raise ValueError("attention weights are tracked for a paged cache")
         if cfg.heads % world or cfg.kv_heads % world:
             raise ValueError(f"{cfg.name}: {cfg.heads} query / {cfg.kv_heads} KV heads do not split over {world}")
         if world > 1 and tp is None:
@@ -201,7 +206,16 @@ class Decoder:
         self.hq, self.hkv = cfg.heads // world, cfg.kv_heads // world
         self.max_seq = context_len + max_new
         self.context_len = context_len
+        # paged cache: one pool of pages per layer under one block table, and per
+        # sequence the slots in use and the position of its current token (both on
+        # the device, the token of the step included)
+        self.page_size, self.track = page_size, track
         B = batch
+        if page_size:
+            blocks = -(-self.max_seq // page_size)
+            self.table = torch.arange(B * blocks, dtype=torch.int32, device=dev).view(B, blocks)
+            self.lens = torch.full((B,), context_len + 1, dtype=torch.int32, device=dev)
+            self.positions = torch.full((B,), context_len, dtype=torch.int32, device=dev)
 
         def slot(i, name):  # one seed per tensor, the same in every process
             return (seed * 1000003 + i * 1009 + zlib.crc32(name.encode())) % (1 << 62)
@@ -272,6 +286,8 @@ class Decoder:
             vc = (kv_scale * torch.randn(kvshape, generator=g, device=dev)).to(torch.float16)
             L["k"] = kc[:, hkv0:hkv0 + self.hkv].contiguous()
             L["v"] = vc[:, hkv0:hkv0 + self.hkv].contiguous()
+            if page_size:
+                self._page(L)
             keep((li, "kcache"), kc)
             keep((li, "vcache"), vc)
             del kc, vc
@@ -306,6 +322,11 @@ class Decoder:
         self.logits = z(B, cfg.vocab)
         self.part = z(B, D) if self.col_batch else None  # this rank's partial residual block
         self.tokens = torch.zeros(B, dtype=torch.int32, device=dev)
+        if page_size:
+            cache, slots = self.layers[0]["cache"], self.table.shape[1] * page_size
+            self.kv_scratch = cache.scratch(B, self.hq, slots if track else 0)
+            self.evict_scratch = cache.evict_scratch(B, slots) if track else None
+            self._lens_next = torch.zeros_like(self.lens)
         sbytes = self.lib.kq_dec_attention_scratch(ctx.handle, B, self.hq, self.hkv, hd, self.max_seq)
         self.att_scratch = torch.zeros(max(sbytes // 4, 1), device=dev)  # counters start at zero
         self.att_scratch_bytes = sbytes
@@ -317,6 +338,24 @@ class Decoder:
         order = [L[key] for L in self.layers for key in ("qkv", "o", "gu", "down")] + [self.head]
         self._next = {id(a): b for a, b in zip(order, order[1:] + [None])}
         torch.cuda.synchronize(dev)
+
+    def _page(self, L) -> None:
+        """The layer's contiguous caches laid out in pages, in the block table's order."""
+        import torch
+        B, blocks = self.table.shape
+        P, hd = self.page_size, self.cfg.head_dim
+        for key in ("k", "v"):
+            pool = torch.zeros((B, self.hkv, blocks * P, hd), dtype=torch.float16, device=self.device)
+            pool[:, :, :self.max_seq] = L[key]
+            L[key] = pool.view(B, self.hkv, blocks, P, hd).transpose(1, 2).reshape(
+                B * blocks, self.hkv, P, hd).contiguous()
+        torch.cuda.synchronize(self.device)
+        L["cache"] = paged.PagedCache(self.ctx, L["k"], L["v"])
+        L["mass"] = L["slot_pos"] = None
+        if self.track:
+            L["mass"] = torch.zeros((B, self.hkv, blocks * P), device=self.device)
+            L["slot_pos"] = torch.arange(blocks * P, dtype=torch.int32, device=self.device).expand_as(
+                L["mass"]).contiguous()
 
     # ---- one decode step ------------------------------------------------------------
     def _check(self, rc, what):
@@ -362,14 +401,52 @@ class Decoder:
         self._check(rc, "residual_linear_batch")
         return True
 
-    def step(self, pos: int) -> None:
+    def _rope_attention(self, L, out, out_ld: int, pos: Optional[int]) -> None:
+        """RoPE + append + attention of the step's tokens over the layer's cache."""
+        ptr = lambda t: ctypes.c_void_p(t.data_ptr())  # noqa: E731
+        hd = self.cfg.head_dim
+        if self.page_size:
+            L["cache"].rope_attention(self.qkv, self.table, self.lens, out, self.kv_scratch, theta=self.cfg.theta,
+                                      pos=self.positions, mass=L["mass"], slot_pos=L["slot_pos"])
+            return
+        self._check(self.lib.kq_dec_rope_attention(self.ctx.handle, ptr(self.qkv), self.qkv_ld, ptr(L["k"]),
+                                                   ptr(L["v"]), ptr(out), out_ld, self.batch, self.hq, self.hkv, hd,
+                                                   pos, self.max_seq, self.cfg.theta, ptr(self.att_scratch),
+                                                   self.att_scratch_bytes), "rope_attention")
+
+    def sample(self, u, temperature=None, top_k=None, top_p=None, min_p=None, prob=None, kept=None) -> None:
+        """Queue the draw of the next tokens from ``self.logits`` into
+        ``self.tokens`` (sampling.sample); a row without a possible token gives
+        -1, which the next step embeds as zeros."""
+        sampling.sample(self.ctx, self.logits, u, self.tokens, temperature=temperature, top_k=top_k, top_p=top_p,
+                        min_p=min_p, prob=prob, kept=kept)
+
+    def evict(self, keep: int, recent_from=None) -> None:
+        """Queue the cut of every layer's cache to ``keep`` slots per sequence and
+        kv head by accumulated attention weight (paged.PagedCache.evict); the
+        slots in use, ``self.lens``, follow.  Call it between steps, before
+        ``self.lens`` counts the next token."""
+        if not self.track:
+            raise ValueError("evict needs a decoder made with track=True")
+        for L in self.layers:  # all layers read the same lens: the last one writes them
+            lens_out = self.lens if L is self.layers[-1] else self._lens_next
+            L["cache"].evict(self.table, self.lens, lens_out, L["mass"], L["slot_pos"], L["mass"], L["slot_pos"], keep,
+                             self.evict_scratch, recent_from=recent_from)
+
+    def step(self, pos: Optional[int] = None) -> None:
         """Queue one decode step for the tokens in ``self.tokens`` at position
         ``pos`` (the cache holds positions [0, pos)); logits land in
-        ``self.logits``."""
+        ``self.logits``.  With a paged cache each sequence has a position of its
+        own: ``self.positions[b]`` on the device, in slot ``self.lens[b] - 1``
+        (0: an idle row), both set on the context's stream, and ``pos`` stays
+        None."""
         cfg, lib, c, B = self.cfg, self.lib, self.ctx.handle, self.batch
         D, hd, F = cfg.dim, cfg.head_dim, cfg.ffn
         ptr = lambda t: ctypes.c_void_p(t.data_ptr())  # noqa: E731
-        if not 0 <= pos < self.max_seq:
+        if self.page_size:
+            if pos is not None:
+                raise ValueError("a paged step takes its positions from self.positions")
+        elif pos is None or not 0 <= pos < self.max_seq:
             raise ValueError(f"position {pos} outside the cache ({self.max_seq})")
         if self.step_kernel:
             self._step_persistent(pos)
@@ -384,11 +461,8 @@ class Decoder:
         for L in self.layers:
             self._norm_linear(L["qkv"], L["attn_norm"], self.qkv)
             out, out_ld = (self.attn_r, self.hq * hd) if tp else (self.attn, self.Ap)
-            if self.fused_attention:
-                self._check(lib.kq_dec_rope_attention(c, ptr(self.qkv), self.qkv_ld, ptr(L["k"]), ptr(L["v"]),
-                                                      ptr(out), out_ld, B, self.hq, self.hkv, hd, pos, self.max_seq,
-                                                      cfg.theta, ptr(self.att_scratch), self.att_scratch_bytes),
-                            "rope_attention")
+            if self.page_size or self.fused_attention:
+                self._rope_attention(L, out, out_ld, pos)
             else:
                 self._check(lib.kq_dec_rope_append(c, ptr(self.qkv), self.qkv_ld, ptr(L["k"]), ptr(L["v"]), B,
                                                    self.hq, self.hkv, hd, pos, self.max_seq, cfg.theta), "rope")
@@ -467,10 +541,7 @@ class Decoder:
 
         for L in self.layers:
             reduce_linear(L["qkv"], L["attn_norm"], self.qkv)
-            self._check(lib.kq_dec_rope_attention(c, ptr(self.qkv), self.qkv_ld, ptr(L["k"]), ptr(L["v"]),
-                                                  ptr(self.attn_r), self.hq * hd, 1, self.hq, self.hkv, hd, pos,
-                                                  self.max_seq, cfg.theta, ptr(self.att_scratch),
-                                                  self.att_scratch_bytes), "rope_attention")
+            self._rope_attention(L, self.attn_r, self.hq * hd, pos)
             self._hint(L["o"])
             self._check(lib.kq_dec_tp_partial_linear(tph, L["o"].handle, ptr(self.attn_r), -1, 0), "o partial")
             pending = True
@@ -564,6 +635,8 @@ class Decoder:
             self.lib.kq_step_destroy(self._step)
             self._step = None
         for L in self.layers:
+            if self.page_size:
+                L["cache"].close()
             for key in ("qkv", "o", "gu", "down"):
                 L[key].free()
         self.head.free()
