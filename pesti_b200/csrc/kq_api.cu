@@ -1480,6 +1480,7 @@ int kq_kv_evict(kq_kv* kv, int64_t batch, const int32_t* table, int64_t table_ld
   a.recent_from = recent_from;
   a.keep = keep;
   a.scratch = scratch;
+  a.num_sms = ctx->num_sms;
   a.err = ctx->dev_err;
   DeviceGuard g(ctx->device);
   if (g.status != cudaSuccess) return cuda_fail(ctx, g.status, "cudaSetDevice");

@@ -426,6 +426,7 @@ struct KvEvictArgs {
   const int32_t* recent_from;  // [batch], or NULL: no slot is protected
   int32_t keep;
   void* scratch;
+  int num_sms;
   int* err;
 };
 size_t kv_evict_scratch_bytes(int64_t batch, int hkv, int64_t track_ld);

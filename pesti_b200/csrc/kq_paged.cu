@@ -3,6 +3,7 @@
 // kq_kv_evict).
 #include "kq_paged.cuh"
 
+#include <cooperative_groups.h>
 #include <cuda_fp16.h>
 #include <math.h>
 
@@ -11,11 +12,14 @@
 namespace kq {
 namespace {
 
+namespace cg = cooperative_groups;
+
 // ---- append ---------------------------------------------------------------------
-// One CTA per row: the row's angles once (in 64 bits, hd / 2 of them) into shared
-// memory, then four consecutive pairs of a head per thread and step, AP_STEPS
-// steps' loads in flight.  Bound by the row's bytes: f32 in, f32 q and f16 k, v out.
-constexpr int AP_THREADS = 256, AP_STEPS = 4, AP_MAX_HALF = 128;
+// 32 to 256 threads per row, by its length: the row's angles once (in 64 bits, hd / 2
+// of them) into shared memory, then four consecutive pairs of a head per thread
+// and step, AP_STEPS steps' loads in flight.  Bound by the row's bytes: f32 in,
+// f32 q and f16 k, v out.
+constexpr int AP_THREADS = 256, AP_STEPS = 4;
 
 // Four floats at p, in one access where `vec` (p is then 16-byte aligned).
 __device__ __forceinline__ float4 load4(const float* p, bool vec) {
@@ -36,44 +40,57 @@ __device__ __forceinline__ uint2 halves(float4 v) {
   return make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
 }
 
-__global__ void __launch_bounds__(AP_THREADS) kv_append_kernel(const KvAppendArgs A, bool vec_in, bool vec_out) {
+template <int TPR>
+__global__ void __launch_bounds__(AP_THREADS, 4) kv_append_kernel(const KvAppendArgs A, bool vec_in, bool vec_out) {
   kv_pdl_enter();
-  __shared__ float4 turn_c[AP_MAX_HALF / 4], turn_s[AP_MAX_HALF / 4];
-  const int hd = A.pool.hd, half = hd / 2, hkv = A.pool.hkv, tid = threadIdx.x;
-  const int64_t r = blockIdx.x;
-  const int32_t slot = A.slots[r];
-  if (slot < 0) return;
-  const int64_t b = A.seqs ? A.seqs[r] : r;
-  if (b < 0 || b >= A.batch || slot >= A.table_ld * A.pool.page_size || (A.slot_pos && slot >= A.track_ld)) {
-    if (tid == 0) kv_error(A.err, KV_ERR_ROW);
-    return;
-  }
-  const int32_t page = A.table[b * A.table_ld + slot / A.pool.page_size];
-  const int32_t pos = A.pos ? A.pos[r] : slot;
-  if (tid < half)
-    rope_turn(pos, tid, half, A.log2_theta, reinterpret_cast<float*>(turn_c)[tid], reinterpret_cast<float*>(turn_s)[tid]);
-  const int64_t row0 = kv_row(A.pool, page, slot, 0), head_ld = (int64_t)A.pool.page_size * hd;
-  if (row0 < 0 && tid == 0) kv_error(A.err, KV_ERR_PAGE);
-  __syncthreads();
+  extern __shared__ float4 turns[];  // per row of the CTA: hd / 2 cosines, then as many sines
+  const int hd = A.pool.hd, half = hd / 2, hkv = A.pool.hkv, tid = threadIdx.x % TPR;
+  const int64_t r = (int64_t)blockIdx.x * (AP_THREADS / TPR) + threadIdx.x / TPR;
+  float4* turn_c = turns + (threadIdx.x / TPR) * (half / 2);
+  float4* turn_s = turn_c + half / 4;
+  // q and k heads in quads of pairs (q only where it is wanted); the first steps' loads come
+  // before the row's place is known
   const float* row = A.qkv + r * A.ld;
-  float* q_out = A.q_out ? A.q_out + r * A.q_ld : nullptr;
-  __half* kc = static_cast<__half*>(A.pool.k) + row0;
-  __half* vc = static_cast<__half*>(A.pool.v) + row0;
-  // q and k heads (q only where it is wanted)
-  const int quads = half / 4, first = q_out ? 0 : A.hq * quads, end = (A.hq + hkv) * quads;
-  for (int e0 = first + tid; e0 < end; e0 += AP_STEPS * AP_THREADS) {
-    float4 x[AP_STEPS], y[AP_STEPS];
+  const int quads = half / 4, first = A.q_out ? 0 : A.hq * quads, end = r < A.rows ? (A.hq + hkv) * quads : 0;
+  float4 x[AP_STEPS], y[AP_STEPS];
+  auto load = [&](int e0) {
 #pragma unroll
     for (int k = 0; k < AP_STEPS; ++k) {
-      const int e = e0 + k * AP_THREADS;
+      const int e = e0 + k * TPR;
       if (e >= end) break;
       const float* p = row + (int64_t)(e / quads) * hd + 4 * (e % quads);
       x[k] = load4(p, vec_in);
       y[k] = load4(p + half, vec_in);
     }
+  };
+  load(first + tid);
+  const int32_t slot = r < A.rows ? A.slots[r] : -1;
+  const int64_t b = slot >= 0 && A.seqs ? A.seqs[r] : r;
+  const bool bad = slot >= 0 && (b < 0 || b >= A.batch || slot >= A.table_ld * A.pool.page_size ||
+                                 (A.slot_pos && slot >= A.track_ld));
+  if (bad && tid == 0) kv_error(A.err, KV_ERR_ROW);
+  const bool live = slot >= 0 && !bad;
+  int32_t pos = 0;
+  int64_t row0 = -1;
+  if (live) {
+    const int32_t page = A.table[b * A.table_ld + slot / A.pool.page_size];
+    pos = A.pos ? A.pos[r] : slot;
+    for (int i = tid; i < half; i += TPR)
+      rope_turn(pos, i, half, A.log2_theta, reinterpret_cast<float*>(turn_c)[i], reinterpret_cast<float*>(turn_s)[i]);
+    row0 = kv_row(A.pool, page, slot, 0);
+    if (row0 < 0 && tid == 0) kv_error(A.err, KV_ERR_PAGE);
+  }
+  __syncthreads();
+  if (!live) return;
+  const int64_t head_ld = (int64_t)A.pool.page_size * hd;
+  float* q_out = A.q_out ? A.q_out + r * A.q_ld : nullptr;
+  __half* kc = static_cast<__half*>(A.pool.k) + row0;
+  __half* vc = static_cast<__half*>(A.pool.v) + row0;
+  for (int e0 = first + tid; e0 < end; e0 += AP_STEPS * TPR) {
+    if (e0 != first + tid) load(e0);
 #pragma unroll
     for (int k = 0; k < AP_STEPS; ++k) {
-      const int e = e0 + k * AP_THREADS;
+      const int e = e0 + k * TPR;
       if (e >= end) break;
       const int head = e / quads, i = 4 * (e % quads);
       const float4 c = turn_c[i / 4], s = turn_s[i / 4];
@@ -93,12 +110,12 @@ __global__ void __launch_bounds__(AP_THREADS) kv_append_kernel(const KvAppendArg
     }
   }
   if (row0 < 0) return;
-  for (int e = tid; e < hkv * (hd / 4); e += AP_THREADS) {
+  for (int e = tid; e < hkv * (hd / 4); e += TPR) {
     const int h = e / (hd / 4), i = 4 * (e - h * (hd / 4));
     *reinterpret_cast<uint2*>(vc + h * head_ld + i) = halves(load4(row + (int64_t)(A.hq + hkv + h) * hd + i, vec_in));
   }
   if (A.slot_pos)
-    for (int h = tid; h < hkv; h += AP_THREADS) A.slot_pos[(b * hkv + h) * A.track_ld + slot] = pos;
+    for (int h = tid; h < hkv; h += TPR) A.slot_pos[(b * hkv + h) * A.track_ld + slot] = pos;
 }
 
 // ---- eviction ---------------------------------------------------------------------
@@ -108,13 +125,15 @@ __global__ void __launch_bounds__(AP_THREADS) kv_append_kernel(const KvAppendArg
 // the kept slots above it: the fewest rows move, and no row that is read is
 // written.
 //
-// One CTA selects for a (sequence, kv head): the key of the last slot kept by
-// three passes over 11-bit digits, then the lists of holes and kept slots above
-// by sums over the threads, each owning consecutive slots.  Keys are read from
-// global memory once and stay in shared memory (up to EV_PIECE slots; longer
-// caches go piece by piece).  A second kernel moves the rows: it is bound by
-// them, the first by the latency of its passes.
-constexpr int EV_THREADS = 1024, EV_BINS = 2048, EV_PIECE = 40960;
+// A cluster of up to eight CTAs selects for a (sequence, kv head), each for its
+// share of the slots: the key of the last slot kept by three passes over 11-bit
+// digits whose counts every CTA reads from the others' shared memory, then the
+// lists of holes and kept slots above by sums over the threads, each owning
+// consecutive slots as bits of a mask.  Keys are read from global memory once and
+// stay in shared memory (up to EV_PIECE slots a CTA; longer shares go piece by
+// piece).  A second kernel moves the rows: it is bound by them, the first by the
+// latency of its passes.
+constexpr int EV_THREADS = 512, EV_BINS = 2048, EV_PIECE = 20480, EV_LOADS = 8, EV_MAX_CLUSTER = 8;
 constexpr size_t EV_SMEM = (size_t)EV_PIECE * 4;
 
 // f32 -> unsigned with the same order; -0 as 0, NaN as -inf
@@ -123,25 +142,24 @@ __device__ __forceinline__ uint32_t order_key(float f) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// Exclusive sum over the block (a multiple of 32 threads); `total` gets the sum.
+// Exclusive sum over the block; `total` gets the sum.
 __device__ __forceinline__ int block_scan(int v, int* warp_sums, int& total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  int x = v;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  auto scan = [&](int x) {  // inclusive, over the warp
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, x, o);
-    if (lane >= o) x += y;
-  }
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    return x;
+  };
+  const int x = scan(v);
   __syncthreads();
   if (lane == 31) warp_sums[warp] = x;
   __syncthreads();
-  int before = 0;
-  total = 0;
-  for (int w = 0; w < warps; ++w) {
-    if (w < warp) before += warp_sums[w];
-    total += warp_sums[w];
-  }
-  return before + x - v;
+  const int w = lane < EV_THREADS / 32 ? warp_sums[lane] : 0, upto = scan(w);
+  total = __shfl_sync(0xffffffffu, upto, 31);
+  return __shfl_sync(0xffffffffu, upto - w, warp) + x - v;
 }
 
 struct EvictPlan {  // one (sequence, kv head)
@@ -153,167 +171,244 @@ struct EvictPlan {  // one (sequence, kv head)
 // lie below `keep`, movers above it: together at most track_ld).
 __host__ __device__ __forceinline__ int64_t evict_list(int64_t track_ld) { return (track_ld + 3) & ~int64_t(3); }
 
-__global__ void __launch_bounds__(EV_THREADS) kv_evict_select_kernel(const KvEvictArgs A) {
+struct EvictShared {
+  alignas(16) unsigned hist[EV_BINS];
+  int sums[32];
+  int pick[3];                     // digit, how many of it are kept, how many there are
+  int tot[2][EV_MAX_CLUSTER];      // ties and listed slots of every CTA
+};
+
+__global__ void __launch_bounds__(EV_THREADS, 2) kv_evict_select_kernel(const KvEvictArgs A) {
   extern __shared__ uint32_t keys[];
-  __shared__ unsigned hist[EV_BINS];
-  __shared__ int sums[32];
-  __shared__ int pick[3];  // digit, how many of it are kept, how many there are
-  const int hk = blockIdx.x, hkv = A.pool.hkv, tid = threadIdx.x;
+  __shared__ EvictShared S;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int CL = (int)cluster.num_blocks(), part = (int)cluster.block_rank();
+  const int hk = blockIdx.x / CL, hkv = A.pool.hkv, tid = threadIdx.x;
   const int64_t b = blockIdx.y, bh = b * hkv + hk;
-  for (int e = tid; e < EV_BINS; e += EV_THREADS) hist[e] = 0;
+  for (int e = tid; e < EV_BINS; e += EV_THREADS) S.hist[e] = 0;
   __syncthreads();
   kv_pdl_enter();
   bool bad;
   const int len = (int)kv_len(A.lens[b], min(A.table_ld * A.pool.page_size, A.track_ld), &bad);
   if (bad && tid == 0) kv_error(A.err, KV_ERR_LEN);
   const int keep = A.keep, new_len = min(len, keep);
+  const int share = (int)(((int64_t)len + CL - 1) / CL), s0 = min(len, part * share), n = min(len, s0 + share) - s0;
   EvictPlan* plan = static_cast<EvictPlan*>(A.scratch) + bh;
   int* list = reinterpret_cast<int*>(static_cast<EvictPlan*>(A.scratch) + A.batch * hkv) + bh * evict_list(A.track_ld);
-  const float* mass = A.mass + bh * A.track_ld;
-  const int32_t* spos = A.slot_pos + bh * A.track_ld;
-  float* mass_out = A.mass_out + bh * A.track_ld;
-  int32_t* pos_out = A.pos_out + bh * A.track_ld;
+  const float* mass = A.mass + bh * A.track_ld + s0;
+  const int32_t* spos = A.slot_pos + bh * A.track_ld + s0;
+  float* mass_out = A.mass_out + bh * A.track_ld + s0;
+  int32_t* pos_out = A.pos_out + bh * A.track_ld + s0;
   const int64_t since = A.recent_from ? A.recent_from[b] : INT64_MAX;
   // what stays in place; the holes among it are filled by the second kernel
-#pragma unroll 4
-  for (int i = tid; i < new_len; i += EV_THREADS) {
-    const float m = mass[i];
-    const int32_t p = spos[i];
+  auto stays_put = [&](int i, float m, int32_t p) {
+    if (s0 + i >= new_len) return;
     mass_out[i] = m;
     pos_out[i] = p;
-  }
+  };
+  auto key_of = [&](float m, int32_t p) { return p >= since ? 0xffffffffu : order_key(m); };
+  // f(slot, mass, position) over this CTA's slots, EV_LOADS of each in flight per thread
+  auto each = [&](auto f) {
+    for (int i = tid; i < n; i += EV_LOADS * EV_THREADS) {
+      float m[EV_LOADS];
+      int32_t p[EV_LOADS];
+#pragma unroll
+      for (int q = 0; q < EV_LOADS; ++q)
+        if (i + q * EV_THREADS < n) m[q] = mass[i + q * EV_THREADS], p[q] = spos[i + q * EV_THREADS];
+#pragma unroll
+      for (int q = 0; q < EV_LOADS; ++q)
+        if (i + q * EV_THREADS < n) f(i + q * EV_THREADS, m[q], p[q]);
+    }
+  };
   if (len <= keep) {
-    if (tid == 0) *plan = EvictPlan{0, new_len, {0, 0}};
+    each(stays_put);
+    if (part == 0 && tid == 0) *plan = EvictPlan{0, new_len, {0, 0}};
     return;
   }
-  auto key_of = [&](int i) { return spos[i] >= since ? 0xffffffffu : order_key(mass[i]); };
-  // the digit at which the count from above reaches `left`
+  // the digit at which all CTAs' count from above reaches `left`
   auto find_digit = [&](int left) {
-    const int d = EV_BINS - 1 - 2 * tid;  // this thread's digits: d, d - 1
-    const int n0 = (int)hist[d], n1 = (int)hist[d - 1];
-    int all;
-    const int before = block_scan(n0 + n1, sums, all);
-    if (before < left && left <= before + n0) pick[0] = d, pick[1] = left - before, pick[2] = n0;
-    if (before + n0 < left && left <= before + n0 + n1) pick[0] = d - 1, pick[1] = left - before - n0, pick[2] = n1;
-    hist[d] = hist[d - 1] = 0;
+    cluster.sync();
+    constexpr int PER = EV_BINS / EV_THREADS;  // this thread's digits, the greatest last: d .. d + PER - 1
+    const int d = EV_BINS - PER - PER * tid;
+    int count[PER] = {}, sum = 0, all;
+    static_assert(PER == 4, "one 16-byte load per CTA");
+    uint4 c[EV_MAX_CLUSTER];
+#pragma unroll
+    for (int r = 0; r < EV_MAX_CLUSTER; ++r)
+      c[r] = r < CL ? *reinterpret_cast<const uint4*>(cluster.map_shared_rank(S.hist, r) + d) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int r = 0; r < EV_MAX_CLUSTER; ++r) {
+      count[0] += (int)c[r].x;
+      count[1] += (int)c[r].y;
+      count[2] += (int)c[r].z;
+      count[3] += (int)c[r].w;
+    }
+#pragma unroll
+    for (int q = 0; q < PER; ++q) sum += count[q];
+    int before = block_scan(sum, S.sums, all);
+#pragma unroll
+    for (int q = PER - 1; q >= 0; --q) {
+      if (before < left && left <= before + count[q])
+        S.pick[0] = d + q, S.pick[1] = left - before, S.pick[2] = count[q];
+      before += count[q];
+    }
+    cluster.sync();  // every CTA has read the counts
+    *reinterpret_cast<uint4*>(S.hist + d) = make_uint4(0, 0, 0, 0);
     __syncthreads();
   };
-  const bool whole = len <= EV_PIECE;
-#pragma unroll 4
-  for (int i = tid; i < len; i += EV_THREADS) {
-    const uint32_t k = key_of(i);
+  const bool whole = n <= EV_PIECE;
+  each([&](int i, float m, int32_t p) {
+    const uint32_t k = key_of(m, p);
     if (whole) keys[i] = k;
-    atomicAdd(&hist[k >> 21], 1u);
-  }
-  __syncthreads();
+    atomicAdd(&S.hist[k >> 21], 1u);
+    stays_put(i, m, p);
+  });
   find_digit(keep);
-  uint32_t thr = (uint32_t)pick[0] << 21;  // kept: keys above, and the first `quota` slots of this key
-  int quota = pick[1], tied = pick[2];
+  uint32_t thr = (uint32_t)S.pick[0] << 21;  // kept: keys above, and the first `quota` slots of this key
+  int quota = S.pick[1], tied = S.pick[2];
 #pragma unroll
   for (int shift = 10; shift >= 0 && quota < tied; shift -= 10) {  // (a digit kept whole needs no more)
     const int up = shift + 11 - (shift == 0);
-    for (int i = tid; i < len; i += EV_THREADS) {
-      const uint32_t k = whole ? keys[i] : key_of(i);
-      if (k >> up == thr >> up) atomicAdd(&hist[(k >> shift) & ((1u << (up - shift)) - 1)], 1u);
-    }
-    __syncthreads();
-    find_digit(quota);
-    thr |= (uint32_t)pick[0] << shift;
-    quota = pick[1];
-    tied = pick[2];
-    __syncthreads();
-  }
-  const bool all_ties = quota == tied;  // then thr may be the least key of a digit kept whole: all from it up stay
-  int ties = 0, listed = 0;             // running counts over the slots so far
-  for (int p0 = 0; p0 < len; p0 += EV_PIECE) {
-    const int n = min(EV_PIECE, len - p0), c = ((n + EV_THREADS - 1) / EV_THREADS) | 1;
-    if (!whole) {
-      __syncthreads();
-      for (int i = tid; i < n; i += EV_THREADS) keys[i] = key_of(p0 + i);
-    }
-    __syncthreads();
-    const int i0 = min(n, tid * c), i1 = min(n, i0 + c);  // this thread's slots (c odd: no bank is hit twice)
-    int rank = 0, total;
-    if (!all_ties) {
-      int mine = 0;
-      for (int i = i0; i < i1; ++i) mine += keys[i] == thr;
-      rank = ties + block_scan(mine, sums, total);
-      ties += total;
-    }
-    const int rank0 = rank;
-    // holes below `keep`, kept slots above it
-    auto moves = [&](int i) {
-      const uint32_t k = keys[i];
-      const bool stay = k > thr || (k == thr && (all_ties || rank++ < quota));
-      return stay == (p0 + i >= keep);
+    auto count = [&](uint32_t k) {
+      if (k >> up == thr >> up) atomicAdd(&S.hist[(k >> shift) & ((1u << (up - shift)) - 1)], 1u);
     };
-    int mine = 0;
-    for (int i = i0; i < i1; ++i) mine += moves(i);
-    int at = listed + block_scan(mine, sums, total);
-    listed += total;
-    rank = rank0;
-    for (int i = i0; i < i1; ++i)
-      if (moves(i)) list[at++] = p0 + i;
+    if (whole) {
+#pragma unroll 4
+      for (int i = tid; i < n; i += EV_THREADS) count(keys[i]);
+    } else {
+      each([&](int, float m, int32_t p) { count(key_of(m, p)); });
+    }
+    find_digit(quota);
+    thr |= (uint32_t)S.pick[0] << shift;
+    quota = S.pick[1];
+    tied = S.pick[2];
   }
-  if (tid == 0) *plan = EvictPlan{listed / 2, new_len, {0, 0}};
+  // This thread's slots of a piece (c <= 41 of them, odd: no bank is hit twice), and
+  // the masks of their keys above and at the threshold
+  struct Masks {
+    int first, n;
+    uint64_t above, at_thr;
+  };
+  auto masks_of = [&](int p0, int rest) {
+    const int c = ((rest + EV_THREADS - 1) / EV_THREADS) | 1;
+    const int i0 = min(rest, tid * c), m = min(rest, i0 + c) - i0;
+    Masks x{p0 + i0, m, 0, 0};
+#pragma unroll 4
+    for (int j = 0; j < m; ++j) {
+      const uint32_t k = keys[i0 + j];
+      x.above |= (uint64_t)(k > thr) << j;
+      x.at_thr |= (uint64_t)(k == thr) << j;
+    }
+    return x;
+  };
+  Masks only{};
+  if (whole) only = masks_of(0, n);
+  // f(masks) piece by piece
+  auto pieces = [&](auto f) {
+    if (whole) {
+      f(only);
+      return;
+    }
+    for (int p0 = 0; p0 < n; p0 += EV_PIECE) {
+      const int rest = min(EV_PIECE, n - p0);
+      __syncthreads();
+      for (int i = tid; i < rest; i += EV_THREADS) keys[i] = key_of(mass[p0 + i], spos[p0 + i]);
+      __syncthreads();
+      f(masks_of(p0, rest));
+    }
+  };
+  // Where a CTA's first tie and its first listed slot stand among all: the counts
+  // of the CTAs before it.
+  auto before_here = [&](int k, int mine) {
+    if (tid < CL) cluster.map_shared_rank(&S, tid)->tot[k][part] = mine;
+    cluster.sync();
+    int sum = 0;
+    for (int r = 0; r < part; ++r) sum += S.tot[k][r];
+    return sum;
+  };
+  const bool all_ties = quota == tied;  // then thr may be the least key of a digit kept whole: all from it up stay
+  int ties = 0, total;
+  if (!all_ties) {
+    int here = 0;
+    pieces([&](Masks x) {
+      block_scan(__popcll(x.at_thr), S.sums, total);
+      here += total;
+    });
+    ties = before_here(0, here);
+  }
+  // the slots that move: holes below `keep`, kept slots above it
+  auto movers = [&](auto f) {
+    int seen = ties;
+    pieces([&](Masks x) {
+      if (!all_ties) {  // only the first `quota` of the ties
+        const int left = quota - seen - block_scan(__popcll(x.at_thr), S.sums, total);
+        seen += total;
+        for (int drop = __popcll(x.at_thr) - max(left, 0); drop > 0; --drop)
+          x.at_thr &= ~(1ull << (63 - __clzll((long long)x.at_thr)));
+      }
+      const uint64_t below = (1ull << max(0, min(x.n, keep - s0 - x.first))) - 1;  // slots below `keep`
+      f(s0 + x.first, ((1ull << x.n) - 1) & ((x.above | x.at_thr) ^ below));
+    });
+  };
+  int here = 0;
+  movers([&](int, uint64_t moves) {
+    block_scan(__popcll(moves), S.sums, total);
+    here += total;
+  });
+  int listed = before_here(1, here);
+  movers([&](int i0, uint64_t moves) {
+    int at = listed + block_scan(__popcll(moves), S.sums, total);
+    listed += total;
+    for (; moves; moves &= moves - 1) list[at++] = i0 + __ffsll((long long)moves) - 1;
+  });
+  if (part == CL - 1 && tid == 0) *plan = EvictPlan{listed / 2, new_len, {0, 0}};
 }
 
-// A thread moves one 16-byte piece of K and of V for EV_MOVES rows at a time.
-constexpr int EV_MOVES = 4;
-__global__ void __launch_bounds__(256) kv_evict_move_kernel(const KvEvictArgs A) {
+// A warp moves EV_ROWS rows at a time: half its lanes find where they come from,
+// half where they go, then every lane carries 16-byte pieces of K and V.
+constexpr int EV_ROWS = 16, EV_MOVERS = 256;
+__global__ void __launch_bounds__(EV_MOVERS, 4) kv_evict_move_kernel(const KvEvictArgs A) {
   kv_pdl_enter();
-  const int hk = blockIdx.y, hkv = A.pool.hkv;
+  const int hk = blockIdx.y, hkv = A.pool.hkv, lane = threadIdx.x & 31;
   const int64_t b = blockIdx.z, bh = b * hkv + hk;
   const EvictPlan plan = static_cast<const EvictPlan*>(A.scratch)[bh];
   const int* holes = reinterpret_cast<const int*>(static_cast<const EvictPlan*>(A.scratch) + A.batch * hkv) +
                      bh * evict_list(A.track_ld);
-  const int* movers = holes + plan.moves;
   if (blockIdx.x == 0 && hk == 0 && threadIdx.x == 0) A.lens_out[b] = plan.new_len;
-  const int ch = A.pool.hd / 8, rows = 256 / ch;  // 16-byte pieces of a row; rows the CTA takes at once
-  const int c = threadIdx.x % ch, r = threadIdx.x / ch;
+  const int pieces = A.pool.hd / 8, log2_row = 32 - __clz(pieces);  // of K (a power of two); as many of V
   const int32_t* table = A.table + b * A.table_ld;
-  __half* k = static_cast<__half*>(A.pool.k) + 8 * c;
-  __half* v = static_cast<__half*>(A.pool.v) + 8 * c;
-  for (int m0 = blockIdx.x * rows * EV_MOVES; m0 < plan.moves; m0 += gridDim.x * rows * EV_MOVES) {
-    int dst[EV_MOVES], src[EV_MOVES];
-    int64_t to[EV_MOVES], from[EV_MOVES];
-#pragma unroll
-    for (int q = 0; q < EV_MOVES; ++q) {
-      const int m = m0 + q * rows + r;
-      dst[q] = m < plan.moves ? holes[m] : -1;
-      src[q] = m < plan.moves ? movers[m] : -1;
-    }
-#pragma unroll
-    for (int q = 0; q < EV_MOVES; ++q) {
-      from[q] = to[q] = -1;
-      if (dst[q] < 0) continue;
-      from[q] = kv_row(A.pool, table[src[q] / A.pool.page_size], src[q], hk);
-      to[q] = kv_row(A.pool, table[dst[q] / A.pool.page_size], dst[q], hk);
-      if (from[q] < 0 || to[q] < 0) {
-        kv_error(A.err, KV_ERR_PAGE);
-        dst[q] = -1;
+  const int warps = gridDim.x * (EV_MOVERS / 32);
+  for (int m0 = (blockIdx.x * (EV_MOVERS / 32) + (threadIdx.x >> 5)) * EV_ROWS; m0 < plan.moves; m0 += warps * EV_ROWS) {
+    const int rows = min(EV_ROWS, plan.moves - m0), mine = lane & (EV_ROWS - 1);
+    const bool from = lane >= EV_ROWS;
+    const int slot = mine < rows ? holes[(from ? plan.moves : 0) + m0 + mine] : 0;
+    const int hole = __shfl_xor_sync(0xffffffffu, slot, EV_ROWS);
+    int64_t at = -1;
+    if (mine < rows) {
+      at = kv_row(A.pool, table[slot / A.pool.page_size], slot, hk);
+      if (at < 0) kv_error(A.err, KV_ERR_PAGE);
+      if (from) {  // the mover's weight and position go with its row
+        A.mass_out[bh * A.track_ld + hole] = A.mass[bh * A.track_ld + slot];
+        A.pos_out[bh * A.track_ld + hole] = A.slot_pos[bh * A.track_ld + slot];
       }
     }
-    uint4 kr[EV_MOVES], vr[EV_MOVES];
-    float mass[EV_MOVES];
-    int32_t pos[EV_MOVES];
+    const int all = rows * 2 * pieces;
+    constexpr int AHEAD = 8;
+    for (int e0 = 0; e0 < all; e0 += 32 * AHEAD) {
+      uint4 v[AHEAD];
+      __half* to[AHEAD];
 #pragma unroll
-    for (int q = 0; q < EV_MOVES; ++q) {
-      if (dst[q] < 0) continue;
-      kr[q] = *reinterpret_cast<const uint4*>(k + from[q]);
-      vr[q] = *reinterpret_cast<const uint4*>(v + from[q]);
-      mass[q] = A.mass[bh * A.track_ld + src[q]];
-      pos[q] = A.slot_pos[bh * A.track_ld + src[q]];
-    }
-#pragma unroll
-    for (int q = 0; q < EV_MOVES; ++q) {
-      if (dst[q] < 0) continue;
-      *reinterpret_cast<uint4*>(k + to[q]) = kr[q];
-      *reinterpret_cast<uint4*>(v + to[q]) = vr[q];
-      if (c == 0) {
-        A.mass_out[bh * A.track_ld + dst[q]] = mass[q];
-        A.pos_out[bh * A.track_ld + dst[q]] = pos[q];
+      for (int q = 0; q < AHEAD; ++q) {
+        const int e = e0 + 32 * q + lane, row = min(e >> log2_row, EV_ROWS - 1), piece = e & (2 * pieces - 1);
+        const int64_t src = __shfl_sync(0xffffffffu, at, EV_ROWS + row), dst = __shfl_sync(0xffffffffu, at, row);
+        __half* pool = static_cast<__half*>(piece < pieces ? A.pool.k : A.pool.v);
+        const int off = 8 * (piece < pieces ? piece : piece - pieces);
+        to[q] = e < all && src >= 0 && dst >= 0 ? pool + dst + off : nullptr;
+        if (to[q]) v[q] = *reinterpret_cast<const uint4*>(pool + src + off);
       }
+#pragma unroll
+      for (int q = 0; q < AHEAD; ++q)
+        if (to[q]) *reinterpret_cast<uint4*>(to[q]) = v[q];
     }
   }
 }
@@ -323,7 +418,18 @@ __global__ void __launch_bounds__(256) kv_evict_move_kernel(const KvEvictArgs A)
 cudaError_t kv_append(const KvAppendArgs& a, cudaStream_t s) {
   const bool vec_in = reinterpret_cast<uintptr_t>(a.qkv) % 16 == 0 && a.ld % 4 == 0;
   const bool vec_out = reinterpret_cast<uintptr_t>(a.q_out) % 16 == 0 && a.q_ld % 4 == 0;
-  return launch_pdl(kv_append_kernel, dim3((unsigned)a.rows), dim3(AP_THREADS), 0, s, a, vec_in, vec_out);
+  // about AP_STEPS steps a thread
+  const int hd = a.pool.hd;
+  const int64_t steps = ((a.q_out ? a.hq : 0) + a.pool.hkv) * (hd / 8) + a.pool.hkv * (hd / 4);
+  auto launch = [&](auto kernel, int tpr) {
+    const int rows = AP_THREADS / tpr;
+    return launch_pdl(kernel, dim3((unsigned)((a.rows + rows - 1) / rows)), dim3(AP_THREADS),
+                      (size_t)rows * hd * sizeof(float), s, a, vec_in, vec_out);
+  };
+  if (steps <= 32 * AP_STEPS) return launch(kv_append_kernel<32>, 32);
+  if (steps <= 64 * AP_STEPS) return launch(kv_append_kernel<64>, 64);
+  if (steps <= 128 * AP_STEPS) return launch(kv_append_kernel<128>, 128);
+  return launch(kv_append_kernel<256>, 256);
 }
 
 size_t kv_evict_scratch_bytes(int64_t batch, int hkv, int64_t track_ld) {
@@ -336,15 +442,32 @@ cudaError_t kv_evict_init_device() {
 
 cudaError_t kv_evict(const KvEvictArgs& a, int* launches, cudaStream_t s) {
   const int64_t most = std::min(a.track_ld, a.table_ld * a.pool.page_size);  // slots a sequence may have
-  const size_t smem = (size_t)std::min<int64_t>(most, EV_PIECE) * 4;
-  cudaError_t e = launch_pdl(kv_evict_select_kernel, dim3((unsigned)a.pool.hkv, (unsigned)a.batch), dim3(EV_THREADS),
-                             smem, s, a);
+  const int64_t pairs = a.batch * a.pool.hkv;
+  // more CTAs per pair while each has over eight slots a thread and SMs are left (two
+  // barriers of the cluster per digit cost what a CTA alone needs for about as many)
+  int cl = 1;
+  while (cl < EV_MAX_CLUSTER && most > cl * 8 * EV_THREADS && pairs * cl <= a.num_sms) cl *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(a.pool.hkv * cl), (unsigned)a.batch);
+  cfg.blockDim = dim3(EV_THREADS);
+  cfg.dynamicSmemBytes = (size_t)std::min<int64_t>((most + cl - 1) / cl, EV_PIECE) * 4;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)cl;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kv_evict_select_kernel, a);
   if (e != cudaSuccess) return e;
+  // a warp per EV_ROWS rows, up to about eight CTAs per SM over all pairs
   const int64_t moves = std::min<int64_t>(a.keep, std::max<int64_t>(0, most - a.keep));
-  const int64_t per_cta = 256 / (a.pool.hd / 8) * EV_MOVES;
-  const unsigned ctas = (unsigned)std::max<int64_t>(1, std::min<int64_t>((moves + per_cta - 1) / per_cta, 64));
+  const int64_t per_cta = EV_MOVERS / 32 * EV_ROWS, cap = std::max<int64_t>(1, 8 * a.num_sms / pairs);
+  const unsigned ctas = (unsigned)std::max<int64_t>(1, std::min<int64_t>((moves + per_cta - 1) / per_cta, cap));
   *launches = 1;
-  e = launch_pdl(kv_evict_move_kernel, dim3(ctas, (unsigned)a.pool.hkv, (unsigned)a.batch), dim3(256), 0, s, a);
+  e = launch_pdl(kv_evict_move_kernel, dim3(ctas, (unsigned)a.pool.hkv, (unsigned)a.batch), dim3(EV_MOVERS), 0, s, a);
   *launches += e == cudaSuccess;
   return e;
 }

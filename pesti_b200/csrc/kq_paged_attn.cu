@@ -757,21 +757,29 @@ __global__ void __launch_bounds__(PaCfg<HD, NS>::THREADS, PaCfg<HD, NS>::CTAS)
 __global__ void __launch_bounds__(256) kv_mass_kernel(const __grid_constant__ PaParams P) {
   kv_pdl_enter();
   const KvAttnArgs& A = P.a;
+  __shared__ float2 stats[KV_MAX_GROUP];  // {max, 1 / sum}
   const int hk = blockIdx.y;
   const int64_t b = blockIdx.z, bh = b * A.pool.hkv + hk;
+  const char* scratch = static_cast<const char*>(A.scratch);
+  if (threadIdx.x < P.G) {
+    const float2 ml = (reinterpret_cast<const float2*>(scratch + P.at.stats) + b * A.hq + hk * P.G)[threadIdx.x];
+    stats[threadIdx.x] = make_float2(ml.x, 1.f / ml.y);
+  }
   bool bad;
   const int len = pa_len(A, b, &bad);
-  const char* scratch = static_cast<const char*>(A.scratch);
-  const float2* stats = reinterpret_cast<const float2*>(scratch + P.at.stats) + b * A.hq + hk * P.G;
-  const float* scores = reinterpret_cast<const float*>(scratch + P.at.scores) + bh * A.track_ld * P.gp;
+  __syncthreads();
+  const float2* scores = reinterpret_cast<const float2*>(scratch + P.at.scores) + bh * A.track_ld * (P.gp / 2);
   float* mass = A.mass + bh * A.track_ld;
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < len; i += (int64_t)gridDim.x * blockDim.x) {
+    const float old = A.rope && i == len - 1 ? 0.f : mass[i];
     float v = 0.f;
-    for (int h = 0; h < P.G; ++h) {
-      const float2 ml = stats[h];
-      v += ex2(scores[i * P.gp + h] - ml.x) / ml.y;
+#pragma unroll 4
+    for (int h = 0; h < P.G; h += 2) {
+      const float2 s = scores[i * (P.gp / 2) + h / 2];
+      v += ex2(s.x - stats[h].x) * stats[h].y;
+      if (h + 1 < P.G) v += ex2(s.y - stats[h + 1].x) * stats[h + 1].y;
     }
-    mass[i] = A.rope && i == len - 1 ? v : mass[i] + v;
+    mass[i] = old + v;
   }
 }
 
@@ -836,7 +844,7 @@ cudaError_t kv_attention(const KvAttnArgs& a, const KvMaps& maps, int* launches,
   *launches = 1;
   if (!a.mass) return e;
   const int64_t most = std::min(a.track_ld, a.table_ld * a.pool.page_size);
-  const unsigned chunks = (unsigned)std::min<int64_t>((most + 255) / 256, 64);
+  const unsigned chunks = (unsigned)std::min<int64_t>((most + 511) / 512, 64);
   e = launch_pdl(kv_mass_kernel, dim3(chunks, (unsigned)a.pool.hkv, (unsigned)a.batch), dim3(256), 0, s, P);
   *launches += e == cudaSuccess;
   return e;

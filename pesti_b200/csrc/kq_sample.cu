@@ -79,23 +79,21 @@ static_assert(sizeof(SampleShared) % 16 == 0, "the slice follows");
 template <int NT>
 __device__ __forceinline__ u64 block_scan(u64 v, u64* sums, u64& total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  u64 x = v;
+  auto scan = [&](u64 x) {  // inclusive, over the warp
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const u64 y = __shfl_up_sync(0xffffffffu, x, o);
-    if (lane >= o) x += y;
-  }
+    for (int o = 1; o < 32; o <<= 1) {
+      const u64 y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    return x;
+  };
+  const u64 x = scan(v);
   __syncthreads();
   if (lane == 31) sums[warp] = x;
   __syncthreads();
-  u64 before = 0;
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < NT / 32; ++w) {
-    if (w < warp) before += sums[w];
-    total += sums[w];
-  }
-  return before + x - v;
+  const u64 w = lane < NT / 32 ? sums[lane] : 0, upto = scan(w);
+  total = __shfl_sync(0xffffffffu, upto, 31);
+  return __shfl_sync(0xffffffffu, upto - w, warp) + x - v;
 }
 
 // The weights of one row.

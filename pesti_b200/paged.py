@@ -52,7 +52,7 @@ class PagedCache:
         if not k[0].is_contiguous():
             raise _invalid(f"pool strides {k.stride()}: the pages must be contiguous")
         page_ld = k.stride(0) if self.pages > 1 else k[0].numel()
-        self.device = torch.device("cuda", ctx.device)
+        self.device, self.index = torch.device("cuda", ctx.device), ctx.device
         if k.device != self.device or v.device != self.device:
             raise _invalid(f"pools on {k.device} and {v.device}, context on {self.device}")
         self.ctx, self.k, self.v = ctx, k, v
@@ -63,41 +63,42 @@ class PagedCache:
                                         self.page_size, self.kv_heads, self.head_dim, ctypes.byref(h)), "kq_kv_create")
         self.handle = h
 
-    # ---- argument checks ---------------------------------------------------------------
+    # ---- argument checks (lean: they run before every call) ------------------------------
     def _rows(self, t, name: str, dtype, rows: int = -1):
-        """A matrix (or the flat form of one row) with unit inner stride; its row stride."""
-        if t.dtype != dtype or t.device != self.device or t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
-            raise _invalid(f"{name}: {t.dtype} {tuple(t.shape)} strides {t.stride()} on {t.device}; rows of {dtype} on "
+        """The row stride of a matrix with unit inner stride."""
+        shape, stride = t.shape, t.stride()
+        if t.dtype is not dtype or t.get_device() != self.index or len(shape) != 2 or (stride[1] != 1 and shape[1] > 1):
+            raise _invalid(f"{name}: {t.dtype} {tuple(shape)} strides {stride} on {t.device}; rows of {dtype} on "
                            f"{self.device} are wanted")
-        if 0 <= rows != t.shape[0]:
-            raise _invalid(f"{name}: {t.shape[0]} rows where {rows} are wanted")
-        return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+        if 0 <= rows != shape[0]:
+            raise _invalid(f"{name}: {shape[0]} rows where {rows} are wanted")
+        return stride[0] if shape[0] > 1 else shape[1]
 
     def _vector(self, t, name: str, n: int):
-        """An int32 vector of n values (None stays None)."""
+        """The address of n contiguous int32 (None stays None)."""
         if t is None:
             return None
-        if t.dtype != self._types[1] or t.device != self.device or t.dim() != 1 or t.shape[0] != n or (
-                n > 1 and t.stride(0) != 1):
+        if t.dtype is not self._types[1] or t.get_device() != self.index or t.shape != (n,) or not t.is_contiguous():
             raise _invalid(f"{name}: {t.dtype} {tuple(t.shape)} on {t.device}; {n} contiguous int32 are wanted")
         return t.data_ptr()
 
     def _track(self, t, name: str, dtype, batch: int, ld=None):
-        """A contiguous [batch][kv_heads][track_ld] array (None stays None); its pointer and track_ld."""
+        """The address and track_ld of a contiguous [batch][kv_heads][track_ld] array (None stays None)."""
         if t is None:
             return None, ld or 0
-        if t.dtype != dtype or t.device != self.device or t.dim() != 3 or not t.is_contiguous() or t.shape[:2] != (
-                batch, self.kv_heads):
-            raise _invalid(f"{name}: {t.dtype} {tuple(t.shape)} on {t.device}; contiguous {dtype} [{batch}]"
+        shape = t.shape
+        if t.dtype is not dtype or t.get_device() != self.index or len(shape) != 3 or not t.is_contiguous() or (
+                shape[0] != batch or shape[1] != self.kv_heads):
+            raise _invalid(f"{name}: {t.dtype} {tuple(shape)} on {t.device}; contiguous {dtype} [{batch}]"
                            f"[{self.kv_heads}][slots] is wanted")
-        if ld and ld != t.shape[2]:
-            raise _invalid(f"{name}: {t.shape[2]} slots where the others have {ld}")
-        return t.data_ptr(), t.shape[2]
+        if ld and ld != shape[2]:
+            raise _invalid(f"{name}: {shape[2]} slots where the others have {ld}")
+        return t.data_ptr(), shape[2]
 
     def _scratch(self, t):
-        if t.device != self.device or not t.is_contiguous():
+        if t.get_device() != self.index or not t.is_contiguous():
             raise _invalid(f"scratch on {t.device}: contiguous memory on {self.device} is wanted")
-        return t.data_ptr(), t.numel() * t.element_size()
+        return t.data_ptr(), t.nbytes
 
     # ---- calls -----------------------------------------------------------------------------
     def scratch(self, batch: int, heads: int, track_ld: int = 0):
