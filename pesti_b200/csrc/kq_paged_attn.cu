@@ -41,7 +41,6 @@ using sm100::smem_u32;
 
 constexpr int PA_TILE = 64;     // slots per ring stage
 constexpr int PA_SHIFT = 14;    // P carries 2^14
-constexpr int PA_PARTS = 512;   // CTAs that can share a pair: two per SM
 constexpr int PA_SET = 128;     // threads of the four warps that share a set of eight query heads
 
 template <int HD, int NS>
@@ -49,9 +48,10 @@ struct PaCfg {
   static constexpr int KS = HD / 16;  // k16 steps of a row
   static constexpr int CW = 4 * NS, THREADS = (CW + 1) * 32;
   static constexpr int TILE_B = PA_TILE * HD * 2, STAGE = 2 * TILE_B;
-  // two CTAs per SM where 96 KB of ring each still leaves room for two
-  static constexpr int CTAS = NS == 1 && HD <= 128 ? 2 : 1;
-  static constexpr int STAGES = HD == 256 ? (NS == 1 ? 3 : 2) : (NS == 1 ? 384 : 768) / HD;
+  // Two CTAs per SM where two fit with their rings (measured against more, smaller ones: four for
+  // 64-dim heads take 30.2 us where two take 24.4, 64 sequences of 2049 with 14 / 2 heads)
+  static constexpr int CTAS = HD == 64 || (HD == 128 && NS == 1) ? 2 : 1;
+  static constexpr int STAGES = HD == 64 ? 6 : HD == 128 ? (NS == 1 ? 3 : 6) : (NS == 1 ? 3 : 2);
   static constexpr int QF = STAGES * STAGE;            // q fragments [NS][KS][32] {hi, hi, lo, lo}
   static constexpr int RED = QF + NS * KS * 512;       // [NS][2][8][HD] f32: the warps' sums
   static constexpr int ML = RED + NS * 2 * 8 * HD * 4;  // [NS][4][8] {max, sum}
@@ -60,7 +60,8 @@ struct PaCfg {
   static constexpr int BAR = NEW + NS * 2 * HD * 2;    // full, empty
   static constexpr int LAST = BAR + 2 * STAGES * 8;    // [NS][2] flags
   static constexpr int END = LAST + NS * 8;
-  static_assert(NS * PA_PARTS * 8 * 8 <= QF, "the join's {max, sum} lie in the ring");
+  static constexpr int PARTS = CTAS * 160;  // CTAs at most, and so parts of a pair
+  static_assert(NS * PARTS * 8 * 8 <= QF, "the join's {max, sum} lie in the ring");
   static_assert(END <= 232448 && CTAS * (END + 1024) <= 233472, "shared memory");
 };
 
@@ -106,6 +107,12 @@ __device__ __forceinline__ void pa_mma(float (&d)[4], const uint32_t (&a)[4], ui
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void pa_mma0(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {  // C = 0
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ void pa_ldm(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -161,11 +168,21 @@ struct PaWalk {
     };
     const int first = units(lane);
     int64_t sum = first;
-    for (int64_t i = lane + 32; i < A.batch; i += 32) sum += units(i);
+    int pairs = first > 0;
+    for (int64_t i = lane + 32; i < A.batch; i += 32) {
+      const int n = units(i);
+      sum += n;
+      pairs += n > 0;
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    pairs = __reduce_add_sync(0xffffffffu, pairs);
     total = sum * hkv;
     ctas = (int)min((int64_t)gridDim.x, total);
+    // More CTAs shorten the runs and lengthen the joins (a part read costs about an eighth of a tile):
+    // the sum is least at sqrt(8 tiles / pair) parts a pair.  Measured for one context of 65,536 and
+    // one pair: 45.7, 34.4, 32.7, 34.2, 49.8 us at 1, 4, 8, 16 and no limit; many pairs never reach it.
+    ctas = min(ctas, (int)ceilf(sqrtf(8.f * (float)total * (float)((int64_t)pairs * hkv))));
     f = f1 = 0;
     if ((int)blockIdx.x >= ctas) return;
     f = begin(blockIdx.x);
@@ -324,9 +341,11 @@ __global__ void __launch_bounds__(PaCfg<HD, NS>::THREADS, PaCfg<HD, NS>::CTAS)
     if (bad && tid == 0) kv_error(A.err, KV_ERR_LEN);
   }
 
-  // lane's places in a 16-slot group: rows of K (M rows, two k8 halves) and of V (transposed)
-  const int k_row = (lane & 7) + ((lane >> 3) & 1) * 8, k_ch = lane >> 4;
-  const int v_row = (lane & 7) + (lane >> 4) * 8, v_ch = (lane >> 3) & 1;
+  // lane's places in a 16-slot group, swizzled: rows of K (M rows, two k8 halves) and of V
+  // (transposed); the 16-byte piece 2 kk of a 128-byte row is then one xor away
+  const uint32_t k_row = (lane & 7) + ((lane >> 3) & 1) * 8, v_row = (lane & 7) + (lane >> 4) * 8;
+  const uint32_t k_lane = k_row * 128 + (((lane >> 4) ^ (lane & 7)) << 4);
+  const uint32_t v_lane = v_row * 128 + ((((lane >> 3) & 1) ^ (lane & 7)) << 4);
   const uint32_t box_b = P.box * 128;  // bytes of one 64-dim half of a box
   const uint32_t group_off = (uint32_t)(16 * w / P.box) * P.box * HD * 2 + (uint32_t)(16 * w % P.box) * 128;
   const uint32_t ring = smem_u32(sm) + group_off;
@@ -468,17 +487,22 @@ __global__ void __launch_bounds__(PaCfg<HD, NS>::THREADS, PaCfg<HD, NS>::CTAS)
             __syncwarp();
           }
           // S^T = K q^T: slots g, g + 8; heads 2c, 2c + 1
-          float sa[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}}, sb[4] = {0.f, 0.f, 0.f, 0.f};
+          float sa[2][4], sb[2][4];  // two chains each of q's parts
 #pragma unroll
           for (int kk = 0; kk < C::KS; ++kk) {
             uint32_t a[4];
-            pa_ldm(kt + (kk >> 2) * box_b + k_row * 128 + (((2 * (kk & 3) + k_ch) ^ (k_row & 7)) << 4), a);
+            pa_ldm((kt + k_lane + (kk >> 2) * box_b) ^ ((kk & 3) << 5), a);
             const uint4 f = reinterpret_cast<const uint4*>(qf)[kk * 32 + lane];
-            pa_mma(sa[kk & 1], a, f.x, f.y);
-            pa_mma(sb, a, f.z, f.w);
+            if (kk < 2) {
+              pa_mma0(sa[kk], a, f.x, f.y);
+              pa_mma0(sb[kk], a, f.z, f.w);
+            } else {
+              pa_mma(sa[kk & 1], a, f.x, f.y);
+              pa_mma(sb[kk & 1], a, f.z, f.w);
+            }
           }
-          float s00 = (sa[0][0] + sa[1][0] + sb[0]) * xs0, s01 = (sa[0][1] + sa[1][1] + sb[1]) * xs1;
-          float s10 = (sa[0][2] + sa[1][2] + sb[2]) * xs0, s11 = (sa[0][3] + sa[1][3] + sb[3]) * xs1;
+          auto sum = [&](int i) { return sa[0][i] + sa[1][i] + (sb[0][i] + sb[1][i]); };
+          float s00 = sum(0) * xs0, s01 = sum(1) * xs1, s10 = sum(2) * xs0, s11 = sum(3) * xs1;
           if (A.mass && h0 + 2 * c < P.gp) {
             float* sp = scores + (bh * A.track_ld + slot0) * P.gp + h0 + 2 * c;
             if (g < rows) *reinterpret_cast<float2*>(sp + (int64_t)g * P.gp) = make_float2(s00, s01);
@@ -526,18 +550,18 @@ __global__ void __launch_bounds__(PaCfg<HD, NS>::THREADS, PaCfg<HD, NS>::CTAS)
           // O^T += V^T P^T: the tile's product by itself, then a rounded add (the tensor
           // cores cut off what they add to: over a long context that would be a bias)
           auto pv = [&](float (&to)[4], const uint32_t (&a)[4]) {
-            float x[4] = {0.f, 0.f, 0.f, 0.f};
-            pa_mma(x, a, pl0, pl1);
+            float x[4];
+            pa_mma0(x, a, pl0, pl1);
             pa_mma(x, a, ph0, ph1);
 #pragma unroll
             for (int k = 0; k < 4; ++k) to[k] += x[k];
           };
-          const uint32_t va = vt + v_row * 128;
+          const uint32_t va = vt + v_lane;
           if (rows == 16) {
 #pragma unroll
             for (int mt = 0; mt < C::KS; ++mt) {
               uint32_t a[4];
-              pa_ldm_t(va + (mt >> 2) * box_b + (((2 * (mt & 3) + v_ch) ^ (v_row & 7)) << 4), a);
+              pa_ldm_t((va + (mt >> 2) * box_b) ^ ((mt & 3) << 5), a);
               pv(o[mt], a);
             }
           } else {
@@ -546,7 +570,7 @@ __global__ void __launch_bounds__(PaCfg<HD, NS>::THREADS, PaCfg<HD, NS>::CTAS)
 #pragma unroll
             for (int mt = 0; mt < C::KS; ++mt) {
               uint32_t a[4];
-              pa_ldm_t(va + (mt >> 2) * box_b + (((2 * (mt & 3) + v_ch) ^ (v_row & 7)) << 4), a);
+              pa_ldm_t((va + (mt >> 2) * box_b) ^ ((mt & 3) << 5), a);
               a[0] &= z0;
               a[1] &= z0;
               a[2] &= z1;
@@ -689,7 +713,7 @@ __global__ void __launch_bounds__(PaCfg<HD, NS>::THREADS, PaCfg<HD, NS>::CTAS)
     // every part's {max, sum} into the ring (its copies are used up); while they
     // come, the first sums: a thread takes a float4 column of parts pg, pg + np, ...
     const int cols = nh * (HD / 4), np = max(1, PA_SET / cols);
-    float2* ml_p = reinterpret_cast<float2*>(sm) + set * PA_PARTS * 8;
+    float2* ml_p = reinterpret_cast<float2*>(sm) + set * C::PARTS * 8;
     for (int e = stid; e < parts * nh; e += PA_SET) ml_p[e] = __ldcg(part_ml + place(e / nh) + e % nh);
     constexpr int AHEAD = 16;
     for (int e = stid; e < (np > 1 ? PA_SET : (cols + PA_SET - 1) / PA_SET * PA_SET); e += PA_SET) {
@@ -788,7 +812,7 @@ cudaError_t launch_attn(const PaParams& P, const KvMaps& maps, int num_sms, cuda
   using C = PaCfg<HD, NS>;
   const KvAttnArgs& a = P.a;
   const int64_t tiles = a.batch * a.pool.hkv * ((a.table_ld * a.pool.page_size + PA_TILE - 1) / PA_TILE);
-  const unsigned grid = (unsigned)std::min<int64_t>(std::min<int64_t>(C::CTAS * num_sms, PA_PARTS), tiles);
+  const unsigned grid = (unsigned)std::min<int64_t>(std::min<int64_t>(C::CTAS * num_sms, C::PARTS), tiles);
   return launch_pdl(kv_attn_kernel<HD, NS>, dim3(grid), dim3(C::THREADS), C::END, s, maps.k, maps.v, P);
 }
 
