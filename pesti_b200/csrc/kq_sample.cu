@@ -41,7 +41,7 @@ constexpr int SM_BINS = 2048;
 constexpr int SM_LIST = 1024;  // candidates one CTA ranks
 constexpr int SM_MAX_CLUSTER = 8;
 constexpr int SM_SLICE = SAMPLE_MAX_VOCAB / SM_MAX_CLUSTER;  // logits a CTA can hold
-constexpr int SM_POW = 256;
+constexpr int SM_POW = 256;  // (2^8 entries of 2^20 / 2^8 in a double's upper half: the shift by 12 below)
 constexpr int SM_FRAC = 44;  // distances above 31.2 T weigh less than 1/2: 0
 
 // f32 -> unsigned with the same order (-0 as 0)
@@ -63,7 +63,7 @@ struct Cut {
 };
 
 struct SampleShared {
-  double pow2[SM_POW];  // 2^(i / SM_POW)
+  double pow2[SM_POW];  // 2^(frac + i / SM_POW)
   u64 sums[SM_MAX_WARPS];
   u64 tot[2][SM_MAX_CLUSTER], tot2[2][SM_MAX_CLUSTER];  // two values of every CTA of the cluster, two sets in turn
   u64 res[4];                                     // what this CTA found for all
@@ -98,27 +98,31 @@ __device__ __forceinline__ u64 block_scan(u64 v, u64* sums, u64& total) {
 
 // The weights of one row.
 struct Weights {
-  double c, zmax64, far;  // SM_POW log2 e / T, the greatest logit, a distance from which on the weight is 0
-  float zmax, per_t;      // the greatest logit, 128 / T
-  int frac;
-  const double* pow2;
-  __device__ __forceinline__ Weights(float top, float T, int frac_, const double* table)
-      : c(SM_POW * 1.4426950408889634074 / (double)T), zmax64((double)top), far(-31.6 * (double)T), zmax(top),
-        per_t(fminf(128.f / T, FLT_MAX)), frac(frac_), pow2(table) {}
+  double c, zmax64;         // SM_POW log2 e / T, the greatest logit
+  float zmax, per_t, zero;  // the greatest logit, 128 / T, a logit from which on the weight is 0
+  const double* pow2;       // 2^(frac + i / SM_POW)
+  __device__ __forceinline__ Weights(float top, float T, const double* table)
+      : c(SM_POW * 1.4426950408889634074 / (double)T), zmax64((double)top), zmax(top), per_t(fminf(128.f / T, FLT_MAX)),
+        zero(nextafterf(top - 31.6f * T, -INFINITY)), pow2(table) {
+    // Where the logits' steps are far above T (31.6 T below the top is one step), every token below the
+    // top weighs 0: its distance is kept to what the exponent holds.
+    const double most = 46.0 * SM_POW, t = (zmax64 - (double)fmaxf(zero, -FLT_MAX)) * c;
+    if (t > most) c *= most / t;
+  }
   // the bin of the distance from the maximum, 128 per T; the last takes all beyond
   __device__ __forceinline__ int bin(float f) const { return (int)fminf((zmax - f) * per_t, (float)(SM_BINS - 1)); }
   // The weight is e p to about 2e-13: 2^t = 2^(n / 256) 2^r with |r| <= 1/512, a
   // table and the exponential series in r.
   __device__ __forceinline__ void parts(float z, double& e, double& p) const {
     constexpr double ROUND = 6755399441055744.0;  // 1.5 2^52: the sum's last bits are the nearest integer
-    const double d = fmax((double)z - zmax64, far);
+    const double d = (double)fmaxf(z, zero) - zmax64;
     const double nd = fma(d, c, ROUND);
     const double r = fma(d, c, ROUND - nd);
     const int n = __double2loint(nd);
     constexpr double A = 0.69314718055994530942 / SM_POW;
     p = fma(r, fma(r, fma(r, A * A * A / 6, A * A / 2), A), 1.0);
     const double w = pow2[n & (SM_POW - 1)];
-    e = __hiloint2double(__double2hiint(w) + (int)((uint32_t)((n >> 8) + frac) << 20), __double2loint(w));
+    e = __hiloint2double(__double2hiint(w) + (int)((uint32_t)(n & ~(SM_POW - 1)) << 12), __double2loint(w));
   }
   __device__ __forceinline__ double scaled(float z) const {
     double e, p;
@@ -410,10 +414,11 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
   const int i0 = min(A.vocab, rank * slice), n = min(A.vocab, i0 + slice) - i0;  // this CTA's tokens
   float* z = reinterpret_cast<float*>(dyn + sizeof(SampleShared));
   Row<NT> R{cluster, S, z, CL, rank, i0, n};
+  cluster.barrier_arrive();  // this CTA has started
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (tid < 16) {  // 2^(i / 256) = 2^(16 a / 256) 2^(b / 256)
-    S.pow2[16 * tid] = exp2(tid / 16.0);
-    if (tid) S.pow2[tid] = exp2(tid / 256.0);
+    S.pow2[16 * tid] = exp2(frac + tid / 16.0);
+    if (tid) S.pow2[tid] = exp2(frac + tid / 256.0);
   }
   if (tid == 0) S.listed = 0;
   if (tid < 4) z[n + tid] = -INFINITY;
@@ -437,7 +442,8 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
   const double U = (double)A.u[b];
   asm volatile("cp.async.wait_all;" ::: "memory");
   __syncthreads();
-  if (tid >= 16 && tid < SM_POW && tid % 16) S.pow2[tid] = S.pow2[tid & ~15] * S.pow2[tid & 15];
+  if (tid >= 16 && tid < SM_POW && tid % 16)
+    S.pow2[tid] = S.pow2[tid & ~15] * S.pow2[tid & 15] * __hiloint2double((1023 - frac) << 20, 0);
 
   // ---- the greatest logit of the slice, and bounds from below for the K-th: order
   // statistics of the threads' own greatest, by bins of 1/64 ----
@@ -474,7 +480,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
     }
     __syncthreads();
   }
-  cluster.sync();  // every CTA has started: its shared memory may be written
+  cluster.barrier_wait();  // every CTA has started: its shared memory may be written
   R.publish(__float_as_uint(top), (u64)__float_as_uint(S.kth[0]) << 32 | __float_as_uint(S.kth[1]));
   // at least K tokens lie above the K-th of any CTA, and above the least of the ceil(K / CTAs)-th
   float kth = -INFINITY, share = INFINITY;
@@ -515,7 +521,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
     top = 0.f;
     __syncthreads();
   }
-  const Weights W(top, T, frac, S.pow2);
+  const Weights W(top, T, S.pow2);
   // min-p: the least logit that stays
   const float least = M > 0.0 ? W.logit_of(M, (double)T) : -INFINITY;
   auto fixed = [W](float f) { return W.fixed(f); };
@@ -629,12 +635,19 @@ cudaError_t sample_init_device() {
 cudaError_t dec_sample(const SampleArgs& a, int num_sms, cudaStream_t s) {
   int bits = 0;
   while ((1 << bits) < a.vocab) ++bits;
-  // as many CTAs per row as the slices ask for, and more while a slice has over
-  // two tokens a thread
+  // CTAs per row: as many as the slices ask for, more while every CTA has an SM to
+  // itself (clusters of eight pack badly: half the SMs) and over two tokens a
+  // thread.  Measured at 32 rows of 151,936 under top-p: 47.3 us for four, 49.6 for
+  // eight; at 8 rows 45.9 and 30.5.  Where not even the least number fits so, eight
+  // narrow CTAs, two per SM (64 rows without a filter: 44.7 us, four wide ones 46.8).
   int cl = 1;
-  while (cl < SM_MAX_CLUSTER && (a.vocab > cl * SM_SLICE || a.vocab > cl * 1024)) cl *= 2;
+  while (a.vocab > cl * SM_SLICE) cl *= 2;
+  const auto fits = [&](int n) { return a.batch * n <= (n == 8 ? num_sms / 2 : num_sms); };
+  if (!fits(cl) && cl > 1) cl = SM_MAX_CLUSTER;
+  while (cl < SM_MAX_CLUSTER && a.vocab > cl * 1024 && fits(2 * cl)) cl *= 2;
   const int slice = ((a.vocab + cl - 1) / cl + 3) & ~3;  // whole quads
-  const bool wide = a.batch * cl <= num_sms;             // each CTA has an SM to itself
+  // 1024 threads where a slice is long enough to hide in them and the SM is free
+  const bool wide = fits(cl) && slice > 12288;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.batch * cl));
   cfg.blockDim = dim3(wide ? 1024 : 512);
