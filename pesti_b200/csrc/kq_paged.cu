@@ -15,11 +15,14 @@ namespace {
 namespace cg = cooperative_groups;
 
 // ---- append ---------------------------------------------------------------------
-// 32 to 256 threads per row, by its length: the row's angles once (in 64 bits, hd / 2
-// of them) into shared memory, then four consecutive pairs of a head per thread
-// and step, AP_STEPS steps' loads in flight.  Bound by the row's bytes: f32 in,
-// f32 q and f16 k, v out.
-constexpr int AP_THREADS = 256, AP_STEPS = 4;
+// 16 to 256 threads per row, by its length: the row's angles once (in 64 bits, hd / 2
+// of them, from frequencies that the CTA works out before its rows arrive) into
+// shared memory, then four consecutive pairs of a head per thread and step.  Bound
+// by the row's bytes: f32 in, f32 q and f16 k, v out.  Many small CTAs hide the chain
+// slot - page - row better than several steps' loads in flight: 4099 rows of 32 / 8
+// heads of 128 take 33.2 us with one step and eight CTAs per SM (5569 GB/s), 38.9
+// with four steps and four.
+constexpr int AP_THREADS = 256, AP_MAX_HALF = 128;
 
 // Four floats at p, in one access where `vec` (p is then 16-byte aligned).
 __device__ __forceinline__ float4 load4(const float* p, bool vec) {
@@ -41,27 +44,26 @@ __device__ __forceinline__ uint2 halves(float4 v) {
 }
 
 template <int TPR>
-__global__ void __launch_bounds__(AP_THREADS, 4) kv_append_kernel(const KvAppendArgs A, bool vec_in, bool vec_out) {
-  kv_pdl_enter();
+__global__ void __launch_bounds__(AP_THREADS, 8) kv_append_kernel(const KvAppendArgs A, bool vec_in, bool vec_out) {
   extern __shared__ float4 turns[];  // per row of the CTA: hd / 2 cosines, then as many sines
+  __shared__ double freq[AP_MAX_HALF];
   const int hd = A.pool.hd, half = hd / 2, hkv = A.pool.hkv, tid = threadIdx.x % TPR;
+  if (threadIdx.x < half) freq[threadIdx.x] = rope_freq(threadIdx.x, half, A.log2_theta);
+  __syncthreads();
+  kv_pdl_enter();
   const int64_t r = (int64_t)blockIdx.x * (AP_THREADS / TPR) + threadIdx.x / TPR;
   float4* turn_c = turns + (threadIdx.x / TPR) * (half / 2);
   float4* turn_s = turn_c + half / 4;
-  // q and k heads in quads of pairs (q only where it is wanted); the first steps' loads come
+  // q and k heads in quads of pairs (q only where it is wanted); the first loads come
   // before the row's place is known
   const float* row = A.qkv + r * A.ld;
   const int quads = half / 4, first = A.q_out ? 0 : A.hq * quads, end = r < A.rows ? (A.hq + hkv) * quads : 0;
-  float4 x[AP_STEPS], y[AP_STEPS];
-  auto load = [&](int e0) {
-#pragma unroll
-    for (int k = 0; k < AP_STEPS; ++k) {
-      const int e = e0 + k * TPR;
-      if (e >= end) break;
-      const float* p = row + (int64_t)(e / quads) * hd + 4 * (e % quads);
-      x[k] = load4(p, vec_in);
-      y[k] = load4(p + half, vec_in);
-    }
+  float4 x, y;
+  auto load = [&](int e) {
+    if (e >= end) return;
+    const float* p = row + (int64_t)(e / quads) * hd + 4 * (e % quads);
+    x = load4(p, vec_in);
+    y = load4(p + half, vec_in);
   };
   load(first + tid);
   const int32_t slot = r < A.rows ? A.slots[r] : -1;
@@ -76,7 +78,7 @@ __global__ void __launch_bounds__(AP_THREADS, 4) kv_append_kernel(const KvAppend
     const int32_t page = A.table[b * A.table_ld + slot / A.pool.page_size];
     pos = A.pos ? A.pos[r] : slot;
     for (int i = tid; i < half; i += TPR)
-      rope_turn(pos, i, half, A.log2_theta, reinterpret_cast<float*>(turn_c)[i], reinterpret_cast<float*>(turn_s)[i]);
+      rope_turn(pos, freq[i], reinterpret_cast<float*>(turn_c)[i], reinterpret_cast<float*>(turn_s)[i]);
     row0 = kv_row(A.pool, page, slot, 0);
     if (row0 < 0 && tid == 0) kv_error(A.err, KV_ERR_PAGE);
   }
@@ -86,27 +88,22 @@ __global__ void __launch_bounds__(AP_THREADS, 4) kv_append_kernel(const KvAppend
   float* q_out = A.q_out ? A.q_out + r * A.q_ld : nullptr;
   __half* kc = static_cast<__half*>(A.pool.k) + row0;
   __half* vc = static_cast<__half*>(A.pool.v) + row0;
-  for (int e0 = first + tid; e0 < end; e0 += AP_STEPS * TPR) {
-    if (e0 != first + tid) load(e0);
-#pragma unroll
-    for (int k = 0; k < AP_STEPS; ++k) {
-      const int e = e0 + k * TPR;
-      if (e >= end) break;
-      const int head = e / quads, i = 4 * (e % quads);
-      const float4 c = turn_c[i / 4], s = turn_s[i / 4];
-      const float4 a = make_float4(x[k].x * c.x - y[k].x * s.x, x[k].y * c.y - y[k].y * s.y,
-                                   x[k].z * c.z - y[k].z * s.z, x[k].w * c.w - y[k].w * s.w);
-      const float4 d = make_float4(x[k].x * s.x + y[k].x * c.x, x[k].y * s.y + y[k].y * c.y,
-                                   x[k].z * s.z + y[k].z * c.z, x[k].w * s.w + y[k].w * c.w);
-      if (head < A.hq) {
-        float* o = q_out + (int64_t)head * hd + i;
-        store4(o, a, vec_out);
-        store4(o + half, d, vec_out);
-      } else if (row0 >= 0) {
-        __half* o = kc + (head - A.hq) * head_ld + i;
-        *reinterpret_cast<uint2*>(o) = halves(a);
-        *reinterpret_cast<uint2*>(o + half) = halves(d);
-      }
+  for (int e = first + tid; e < end; e += TPR) {
+    if (e != first + tid) load(e);
+    const int head = e / quads, i = 4 * (e % quads);
+    const float4 c = turn_c[i / 4], s = turn_s[i / 4];
+    const float4 a = make_float4(x.x * c.x - y.x * s.x, x.y * c.y - y.y * s.y, x.z * c.z - y.z * s.z,
+                                 x.w * c.w - y.w * s.w);
+    const float4 d = make_float4(x.x * s.x + y.x * c.x, x.y * s.y + y.y * c.y, x.z * s.z + y.z * c.z,
+                                 x.w * s.w + y.w * c.w);
+    if (head < A.hq) {
+      float* o = q_out + (int64_t)head * hd + i;
+      store4(o, a, vec_out);
+      store4(o + half, d, vec_out);
+    } else if (row0 >= 0) {
+      __half* o = kc + (head - A.hq) * head_ld + i;
+      *reinterpret_cast<uint2*>(o) = halves(a);
+      *reinterpret_cast<uint2*>(o + half) = halves(d);
     }
   }
   if (row0 < 0) return;
@@ -418,7 +415,7 @@ __global__ void __launch_bounds__(EV_MOVERS, 4) kv_evict_move_kernel(const KvEvi
 cudaError_t kv_append(const KvAppendArgs& a, cudaStream_t s) {
   const bool vec_in = reinterpret_cast<uintptr_t>(a.qkv) % 16 == 0 && a.ld % 4 == 0;
   const bool vec_out = reinterpret_cast<uintptr_t>(a.q_out) % 16 == 0 && a.q_ld % 4 == 0;
-  // about AP_STEPS steps a thread
+  // two to four steps a thread
   const int hd = a.pool.hd;
   const int64_t steps = ((a.q_out ? a.hq : 0) + a.pool.hkv) * (hd / 8) + a.pool.hkv * (hd / 4);
   auto launch = [&](auto kernel, int tpr) {
@@ -426,9 +423,10 @@ cudaError_t kv_append(const KvAppendArgs& a, cudaStream_t s) {
     return launch_pdl(kernel, dim3((unsigned)((a.rows + rows - 1) / rows)), dim3(AP_THREADS),
                       (size_t)rows * hd * sizeof(float), s, a, vec_in, vec_out);
   };
-  if (steps <= 32 * AP_STEPS) return launch(kv_append_kernel<32>, 32);
-  if (steps <= 64 * AP_STEPS) return launch(kv_append_kernel<64>, 64);
-  if (steps <= 128 * AP_STEPS) return launch(kv_append_kernel<128>, 128);
+  if (steps <= 16 * 4) return launch(kv_append_kernel<16>, 16);
+  if (steps <= 32 * 4) return launch(kv_append_kernel<32>, 32);
+  if (steps <= 64 * 4) return launch(kv_append_kernel<64>, 64);
+  if (steps <= 128 * 4) return launch(kv_append_kernel<128>, 128);
   return launch(kv_append_kernel<256>, 256);
 }
 

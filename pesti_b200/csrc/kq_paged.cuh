@@ -33,11 +33,15 @@ __device__ __forceinline__ void kv_pdl_enter() {
 
 __device__ __forceinline__ void kv_error(int* err, int code) { atomicCAS(err, 0, code); }
 
+// Turns (of a full circle) per position of pair i: theta^(-i / half) / (2 pi).
+__device__ __forceinline__ double rope_freq(int i, int half, double log2_theta) {
+  return exp2(-(double)i / (double)half * log2_theta) * 0.15915494309189533577;
+}
 // cos / sin of pos * theta^(-i / half).  The angle is reduced in 64 bits: at
 // position 100,000 an f32 angle is off by 4e-3, where the f32 result of this
 // form stays within 1e-7 of the exact one.
-__device__ __forceinline__ void rope_turn(int32_t pos, int i, int half, double log2_theta, float& c, float& s) {
-  const double t = (double)pos * exp2(-(double)i / (double)half * log2_theta) * 0.15915494309189533577;
+__device__ __forceinline__ void rope_turn(int32_t pos, double freq, float& c, float& s) {
+  const double t = (double)pos * freq;
   sincospif(2.f * (float)(t - rint(t)), &s, &c);
 }
 #endif

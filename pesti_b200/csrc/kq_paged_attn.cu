@@ -396,7 +396,7 @@ __global__ void __launch_bounds__(PaCfg<HD, NS>::THREADS, PaCfg<HD, NS>::CTAS)
 #pragma unroll
         for (int k = 0; k < IN; ++k)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) rope_turn(pos, qi + 64 * k + e, HALF, A.log2_theta, cs[k][e], sn[k][e]);
+          for (int e = 0; e < 2; ++e) rope_turn(pos, rope_freq(qi + 64 * k + e, HALF, A.log2_theta), cs[k][e], sn[k][e]);
         turned = W.b;
       }
 #pragma unroll
