@@ -511,6 +511,12 @@ __global__ void __launch_bounds__(PaCfg<HD, NS>::THREADS, PaCfg<HD, NS>::CTAS)
           if (rows < 16) {  // nothing behind the sequence counts, whatever lies there
             if (g >= rows) s00 = s01 = -INFINITY;
             if (g + 8 >= rows) s10 = s11 = -INFINITY;
+            uint8_t* v0 = sm + group_off + s * C::STAGE + C::TILE_B;
+            for (int e = lane; e < (16 - rows) * (HD / 8); e += 32) {
+              const int r = rows + e / (HD / 8), ch = e % (HD / 8);
+              *reinterpret_cast<uint4*>(v0 + (ch >> 3) * box_b + r * 128 + ((ch & 7) << 4)) = make_uint4(0, 0, 0, 0);
+            }
+            __syncwarp();
           }
           float x0 = fmaxf(s00, s10), x1 = fmaxf(s01, s11);
 #pragma unroll
@@ -557,26 +563,11 @@ __global__ void __launch_bounds__(PaCfg<HD, NS>::THREADS, PaCfg<HD, NS>::CTAS)
             for (int k = 0; k < 4; ++k) to[k] += x[k];
           };
           const uint32_t va = vt + v_lane;
-          if (rows == 16) {
 #pragma unroll
-            for (int mt = 0; mt < C::KS; ++mt) {
-              uint32_t a[4];
-              pa_ldm_t((va + (mt >> 2) * box_b) ^ ((mt & 3) << 5), a);
-              pv(o[mt], a);
-            }
-          } else {
-            const uint32_t z0 = (2 * c < rows ? 0xffffu : 0u) | (2 * c + 1 < rows ? 0xffff0000u : 0u);
-            const uint32_t z1 = (2 * c + 8 < rows ? 0xffffu : 0u) | (2 * c + 9 < rows ? 0xffff0000u : 0u);
-#pragma unroll
-            for (int mt = 0; mt < C::KS; ++mt) {
-              uint32_t a[4];
-              pa_ldm_t((va + (mt >> 2) * box_b) ^ ((mt & 3) << 5), a);
-              a[0] &= z0;
-              a[1] &= z0;
-              a[2] &= z1;
-              a[3] &= z1;
-              pv(o[mt], a);
-            }
+          for (int mt = 0; mt < C::KS; ++mt) {
+            uint32_t a[4];
+            pa_ldm_t((va + (mt >> 2) * box_b) ^ ((mt & 3) << 5), a);
+            pv(o[mt], a);
           }
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -628,12 +619,12 @@ __global__ void __launch_bounds__(PaCfg<HD, NS>::THREADS, PaCfg<HD, NS>::CTAS)
 #pragma unroll
           for (int k = 0; k < 4; ++k) o[mt][k] += from[(4 * mt + k) * 32 + lane];
       };
-      if (w >= 2) put(red + (w - 2) * 8 * HD);
-      bar_set(set);
-      if (w < 2) add(red + w * 8 * HD);
-      if (w == 1) put(red + 8 * HD);
-      bar_set(set);
-      if (w == 0) add(red + 8 * HD);
+#pragma unroll 1
+      for (int from = 2; from > 0; from >>= 1) {  // (one copy of the code: what is not fetched costs nothing)
+        if (w >= from && w < 2 * from) put(red + (w & 1) * 8 * HD);
+        bar_set(set);
+        if (w < from) add(red + (from == 2 ? w : 1) * 8 * HD);
+      }
 
       const int64_t out_row = W.b * A.out_ld + (int64_t)(W.hk * P.G + h0) * HD;
       const int head0 = (int)(W.hk * P.G + h0);
@@ -715,7 +706,7 @@ __global__ void __launch_bounds__(PaCfg<HD, NS>::THREADS, PaCfg<HD, NS>::CTAS)
     const int cols = nh * (HD / 4), np = max(1, PA_SET / cols);
     float2* ml_p = reinterpret_cast<float2*>(sm) + set * C::PARTS * 8;
     for (int e = stid; e < parts * nh; e += PA_SET) ml_p[e] = __ldcg(part_ml + place(e / nh) + e % nh);
-    constexpr int AHEAD = 16;
+    constexpr int AHEAD = 8;  // (16 took 1.8 us more of 54 at 32 sequences of 2049: a longer kernel)
     for (int e = stid; e < (np > 1 ? PA_SET : (cols + PA_SET - 1) / PA_SET * PA_SET); e += PA_SET) {
       const int pg = np > 1 ? e / cols : 0, col = np > 1 ? e - pg * cols : e;
       const bool mine = pg < np && col < cols;
