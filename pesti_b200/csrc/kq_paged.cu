@@ -171,8 +171,9 @@ __host__ __device__ __forceinline__ int64_t evict_list(int64_t track_ld) { retur
 struct EvictShared {
   alignas(16) unsigned hist[EV_BINS];
   int sums[32];
-  int pick[3];                     // digit, how many of it are kept, how many there are
-  int tot[2][EV_MAX_CLUSTER];      // ties and listed slots of every CTA
+  int pick[3];                // digit, how many of it are kept, how many there are
+  int sum[EV_MAX_CLUSTER];    // counts of every CTA's digits
+  int tot[2][EV_MAX_CLUSTER];  // ties and listed slots of every CTA
 };
 
 __global__ void __launch_bounds__(EV_THREADS, 2) kv_evict_select_kernel(const KvEvictArgs A) {
@@ -222,36 +223,55 @@ __global__ void __launch_bounds__(EV_THREADS, 2) kv_evict_select_kernel(const Kv
     if (part == 0 && tid == 0) *plan = EvictPlan{0, new_len, {0, 0}};
     return;
   }
-  // the digit at which all CTAs' count from above reaches `left`
+  auto sync_all = [&] {
+    if (CL > 1) cluster.sync();
+    else __syncthreads();
+  };
+  // the digit at which all CTAs' count from above reaches `left`: every CTA joins
+  // the counts of its part of the digits (the first has the greatest), the one in
+  // whose part it lies finds it
   auto find_digit = [&](int left) {
-    cluster.sync();
-    constexpr int PER = EV_BINS / EV_THREADS;  // this thread's digits, the greatest last: d .. d + PER - 1
-    const int d = EV_BINS - PER - PER * tid;
-    int count[PER] = {}, sum = 0, all;
-    static_assert(PER == 4, "one 16-byte load per CTA");
-    uint4 c[EV_MAX_CLUSTER];
+    sync_all();
+    const int digits = EV_BINS / CL, top = EV_BINS - 1 - part * digits;  // this CTA's: [top - digits + 1, top]
+    constexpr int MOST = EV_BINS / EV_THREADS;
+    const int per = (digits + EV_THREADS - 1) / EV_THREADS;
+    int count[MOST] = {}, sum = 0, all;
+    if (CL == 1) {
+      static_assert(MOST == 4, "16 bytes");
+      const uint4 c = reinterpret_cast<const uint4*>(S.hist)[EV_THREADS - 1 - tid];
+      count[0] = (int)c.w, count[1] = (int)c.z, count[2] = (int)c.y, count[3] = (int)c.x;
+    } else {
 #pragma unroll
-    for (int r = 0; r < EV_MAX_CLUSTER; ++r)
-      c[r] = r < CL ? *reinterpret_cast<const uint4*>(cluster.map_shared_rank(S.hist, r) + d) : make_uint4(0, 0, 0, 0);
+      for (int q = 0; q < MOST; ++q) {
+        const int d = top - tid * per - q;
+        if (q >= per || d <= top - digits) continue;
+        unsigned c[EV_MAX_CLUSTER];
 #pragma unroll
-    for (int r = 0; r < EV_MAX_CLUSTER; ++r) {
-      count[0] += (int)c[r].x;
-      count[1] += (int)c[r].y;
-      count[2] += (int)c[r].z;
-      count[3] += (int)c[r].w;
+        for (int r = 0; r < EV_MAX_CLUSTER; ++r) c[r] = r < CL ? cluster.map_shared_rank(S.hist, r)[d] : 0;
+#pragma unroll
+        for (int r = 0; r < EV_MAX_CLUSTER; ++r) count[q] += (int)c[r];
+      }
     }
 #pragma unroll
-    for (int q = 0; q < PER; ++q) sum += count[q];
-    int before = block_scan(sum, S.sums, all);
+    for (int q = 0; q < MOST; ++q) sum += count[q];
+    int before = block_scan(sum, S.sums, all), owner = 0;
+    if (CL > 1) {
+      if (tid < CL) cluster.map_shared_rank(&S, tid)->sum[part] = all;
+      cluster.sync();
+      int upto = S.sum[0];
+      while (upto < left) upto += S.sum[++owner];
+      for (int r = 0; r < part; ++r) before += S.sum[r];
+    }
 #pragma unroll
-    for (int q = PER - 1; q >= 0; --q) {
+    for (int q = 0; q < MOST; ++q) {
       if (before < left && left <= before + count[q])
-        S.pick[0] = d + q, S.pick[1] = left - before, S.pick[2] = count[q];
+        S.pick[0] = top - tid * per - q, S.pick[1] = left - before, S.pick[2] = count[q];
       before += count[q];
     }
-    cluster.sync();  // every CTA has read the counts
-    *reinterpret_cast<uint4*>(S.hist + d) = make_uint4(0, 0, 0, 0);
-    __syncthreads();
+    for (int e = tid; e < EV_BINS; e += EV_THREADS) S.hist[e] = 0;  // (all have read it)
+    sync_all();
+    const int* pick = CL > 1 ? cluster.map_shared_rank(S.pick, owner) : S.pick;
+    return make_int3(pick[0], pick[1], pick[2]);
   };
   const bool whole = n <= EV_PIECE;
   each([&](int i, float m, int32_t p) {
@@ -260,9 +280,9 @@ __global__ void __launch_bounds__(EV_THREADS, 2) kv_evict_select_kernel(const Kv
     atomicAdd(&S.hist[k >> 21], 1u);
     stays_put(i, m, p);
   });
-  find_digit(keep);
-  uint32_t thr = (uint32_t)S.pick[0] << 21;  // kept: keys above, and the first `quota` slots of this key
-  int quota = S.pick[1], tied = S.pick[2];
+  int3 pick = find_digit(keep);
+  uint32_t thr = (uint32_t)pick.x << 21;  // kept: keys above, and the first `quota` slots of this key
+  int quota = pick.y, tied = pick.z;
 #pragma unroll
   for (int shift = 10; shift >= 0 && quota < tied; shift -= 10) {  // (a digit kept whole needs no more)
     const int up = shift + 11 - (shift == 0);
@@ -275,10 +295,10 @@ __global__ void __launch_bounds__(EV_THREADS, 2) kv_evict_select_kernel(const Kv
     } else {
       each([&](int, float m, int32_t p) { count(key_of(m, p)); });
     }
-    find_digit(quota);
-    thr |= (uint32_t)S.pick[0] << shift;
-    quota = S.pick[1];
-    tied = S.pick[2];
+    pick = find_digit(quota);
+    thr |= (uint32_t)pick.x << shift;
+    quota = pick.y;
+    tied = pick.z;
   }
   // This thread's slots of a piece (c <= 41 of them, odd: no bank is hit twice), and
   // the masks of their keys above and at the threshold
@@ -314,9 +334,10 @@ __global__ void __launch_bounds__(EV_THREADS, 2) kv_evict_select_kernel(const Kv
       f(masks_of(p0, rest));
     }
   };
-  // Where a CTA's first tie and its first listed slot stand among all: the counts
-  // of the CTAs before it.
+  // What the CTAs before this one count: where its first tie and its first listed
+  // slot stand among all.
   auto before_here = [&](int k, int mine) {
+    if (CL == 1) return 0;
     if (tid < CL) cluster.map_shared_rank(&S, tid)->tot[k][part] = mine;
     cluster.sync();
     int sum = 0;
@@ -347,17 +368,29 @@ __global__ void __launch_bounds__(EV_THREADS, 2) kv_evict_select_kernel(const Kv
       f(s0 + x.first, ((1ull << x.n) - 1) & ((x.above | x.at_thr) ^ below));
     });
   };
-  int here = 0;
-  movers([&](int, uint64_t moves) {
-    block_scan(__popcll(moves), S.sums, total);
-    here += total;
-  });
-  int listed = before_here(1, here);
-  movers([&](int i0, uint64_t moves) {
-    int at = listed + block_scan(__popcll(moves), S.sums, total);
-    listed += total;
+  int listed = 0;
+  auto write = [&](int i0, uint64_t moves, int at) {
     for (; moves; moves &= moves - 1) list[at++] = i0 + __ffsll((long long)moves) - 1;
-  });
+  };
+  if (whole) {
+    movers([&](int i0, uint64_t moves) {
+      const int at = block_scan(__popcll(moves), S.sums, total);
+      listed = before_here(1, total);
+      write(i0, moves, listed + at);
+      listed += total;
+    });
+  } else {
+    int here = 0;
+    movers([&](int, uint64_t moves) {
+      block_scan(__popcll(moves), S.sums, total);
+      here += total;
+    });
+    listed = before_here(1, here);
+    movers([&](int i0, uint64_t moves) {
+      write(i0, moves, listed + block_scan(__popcll(moves), S.sums, total));
+      listed += total;
+    });
+  }
   if (part == CL - 1 && tid == 0) *plan = EvictPlan{listed / 2, new_len, {0, 0}};
 }
 
