@@ -62,30 +62,32 @@ class PagedCache:
         ctx.check(self.lib.kq_kv_create(ctx.handle, k.data_ptr(), v.data_ptr(), self.pages, page_ld,
                                         self.page_size, self.kv_heads, self.head_dim, ctypes.byref(h)), "kq_kv_create")
         self.handle = h
+        self._append, self._attention = self.lib.kq_kv_append, self.lib.kq_kv_attention
+        self._rope_attention = self.lib.kq_kv_rope_attention
 
     # ---- argument checks (lean: they run before every call) ------------------------------
     def _rows(self, t, name: str, dtype, rows: int = -1):
         """The row stride of a matrix with unit inner stride."""
-        shape, stride = t.shape, t.stride()
-        if t.dtype is not dtype or t.get_device() != self.index or len(shape) != 2 or (stride[1] != 1 and shape[1] > 1):
-            raise _invalid(f"{name}: {t.dtype} {tuple(shape)} strides {stride} on {t.device}; rows of {dtype} on "
-                           f"{self.device} are wanted")
-        if 0 <= rows != shape[0]:
-            raise _invalid(f"{name}: {shape[0]} rows where {rows} are wanted")
-        return stride[0] if shape[0] > 1 else shape[1]
+        try:
+            n, cols = t.shape
+            ld, inner = t.stride()
+            if t.dtype is dtype and t.get_device() == self.index and (inner == 1 or cols <= 1) and (n == rows or rows < 0):
+                return ld if n > 1 else cols
+        except ValueError:  # not a matrix
+            pass
+        raise _invalid(f"{name}: {t.dtype} {tuple(t.shape)} strides {t.stride()} on {t.device}; "
+                       f"{rows if rows >= 0 else 'any'} rows of {dtype} on {self.device} are wanted")
 
     def _vector(self, t, name: str, n: int):
-        """The address of n contiguous int32 (None stays None)."""
-        if t is None:
-            return None
-        if t.dtype is not self._types[1] or t.get_device() != self.index or t.shape != (n,) or not t.is_contiguous():
-            raise _invalid(f"{name}: {t.dtype} {tuple(t.shape)} on {t.device}; {n} contiguous int32 are wanted")
+        """The address of n contiguous int32."""
+        if t is None or t.dtype is not self._types[1] or t.get_device() != self.index or t.shape != (n,) or (
+                not t.is_contiguous()):
+            raise _invalid(f"{name}: {n} contiguous int32 on {self.device} are wanted"
+                           + ("" if t is None else f", not {t.dtype} {tuple(t.shape)} on {t.device}"))
         return t.data_ptr()
 
     def _track(self, t, name: str, dtype, batch: int, ld=None):
-        """The address and track_ld of a contiguous [batch][kv_heads][track_ld] array (None stays None)."""
-        if t is None:
-            return None, ld or 0
+        """The address and track_ld of a contiguous [batch][kv_heads][track_ld] array."""
         shape = t.shape
         if t.dtype is not dtype or t.get_device() != self.index or len(shape) != 3 or not t.is_contiguous() or (
                 shape[0] != batch or shape[1] != self.kv_heads):
@@ -124,39 +126,42 @@ class PagedCache:
         slot slots[r] (-1: none) of sequence seqs[r] (default r), turned to
         position pos[r] (default: the slot); the turned q into q_out."""
         f32, i32 = self._types
-        ld = self._rows(qkv, "qkv", f32)
-        rows, batch = qkv.shape[0], table.shape[0]
-        heads = qkv.shape[1] // self.head_dim - 2 * self.kv_heads
-        if (heads + 2 * self.kv_heads) * self.head_dim != qkv.shape[1]:
-            raise _invalid(f"qkv: rows of {qkv.shape[1]} are not whole heads of {self.head_dim}")
-        q_ld = 0
+        ld, table_ld = self._rows(qkv, "qkv", f32), self._rows(table, "table", i32)
+        rows, cols = qkv.shape
+        batch, hd = table.shape[0], self.head_dim
+        heads = cols // hd - 2 * self.kv_heads
+        if (heads + 2 * self.kv_heads) * hd != cols:
+            raise _invalid(f"qkv: rows of {cols} are not whole heads of {hd}")
+        q_ptr, q_ld = None, 0
         if q_out is not None:
-            q_ld = self._rows(q_out, "q_out", f32, rows)
-            if q_out.shape[1] < heads * self.head_dim:
-                raise _invalid(f"q_out: rows of {q_out.shape[1]} for {heads} heads of {self.head_dim}")
-        sp, track = self._track(slot_pos, "slot_pos", i32, batch)
-        self.ctx.check(self.lib.kq_kv_append(
-            self.handle, qkv.data_ptr(), ld, rows, heads, self._vector(seqs, "seqs", rows),
-            self._vector(slots, "slots", rows), self._vector(pos, "pos", rows), table.data_ptr(),
-            self._rows(table, "table", i32), batch, theta, q_out.data_ptr() if q_out is not None else None, q_ld, sp,
-            track), "kq_kv_append")
+            q_ptr, q_ld = q_out.data_ptr(), self._rows(q_out, "q_out", f32, rows)
+            if q_out.shape[1] < heads * hd:
+                raise _invalid(f"q_out: rows of {q_out.shape[1]} for {heads} heads of {hd}")
+        sp, track = (None, 0) if slot_pos is None else self._track(slot_pos, "slot_pos", i32, batch)
+        rc = self._append(self.handle, qkv.data_ptr(), ld, rows, heads,
+                          None if seqs is None else self._vector(seqs, "seqs", rows),
+                          self._vector(slots, "slots", rows), None if pos is None else self._vector(pos, "pos", rows),
+                          table.data_ptr(), table_ld, batch, theta, q_ptr, q_ld, sp, track)
+        if rc:
+            self.ctx.check(rc, "kq_kv_append")
 
     def attention(self, q, table, lens, out, scratch, mass=None) -> None:
         """out[b] = attention of q[b] [heads][head_dim] (turned already) over
         slots [0, lens[b]) of sequence b (0: zeros); mass accumulates each
         slot's weight, summed over the query heads of its kv head."""
         f32, i32 = self._types
+        q_ld = self._rows(q, "q", f32)
         batch, cols = q.shape
         heads = cols // self.head_dim
-        q_ld, out_ld = self._rows(q, "q", f32), self._rows(out, "out", f32, batch)
+        out_ld = self._rows(out, "out", f32, batch)
         if heads * self.head_dim != cols or out.shape[1] < cols:
             raise _invalid(f"q rows of {cols} and out rows of {out.shape[1]} for heads of {self.head_dim}")
-        m, track = self._track(mass, "mass", f32, batch)
-        sp, sb = self._scratch(scratch)
-        self.ctx.check(self.lib.kq_kv_attention(
-            self.handle, q.data_ptr(), q_ld, out.data_ptr(), out_ld, batch, heads, table.data_ptr(),
-            self._rows(table, "table", i32, batch), self._vector(lens, "lens", batch), m, track, sp, sb),
-            "kq_kv_attention")
+        m, track = (None, 0) if mass is None else self._track(mass, "mass", f32, batch)
+        rc = self._attention(self.handle, q.data_ptr(), q_ld, out.data_ptr(), out_ld, batch, heads, table.data_ptr(),
+                             self._rows(table, "table", i32, batch), self._vector(lens, "lens", batch), m, track,
+                             *self._scratch(scratch))
+        if rc:
+            self.ctx.check(rc, "kq_kv_attention")
 
     def rope_attention(self, qkv, table, lens, out, scratch, *, theta: float, pos=None, mass=None,
                        slot_pos=None) -> None:
@@ -165,18 +170,24 @@ class PagedCache:
         lens[b] - 1, then the attention; the new slot's mass starts anew and its
         position goes to slot_pos."""
         f32, i32 = self._types
+        ld = self._rows(qkv, "qkv", f32)
         batch, cols = qkv.shape
-        heads = cols // self.head_dim - 2 * self.kv_heads
-        ld, out_ld = self._rows(qkv, "qkv", f32), self._rows(out, "out", f32, batch)
-        if (heads + 2 * self.kv_heads) * self.head_dim != cols or out.shape[1] < heads * self.head_dim:
-            raise _invalid(f"qkv rows of {cols} and out rows of {out.shape[1]} for heads of {self.head_dim}")
-        m, track = self._track(mass, "mass", f32, batch)
-        p, track = self._track(slot_pos, "slot_pos", i32, batch, track)
-        sp, sb = self._scratch(scratch)
-        self.ctx.check(self.lib.kq_kv_rope_attention(
-            self.handle, qkv.data_ptr(), ld, out.data_ptr(), out_ld, batch, heads, table.data_ptr(),
-            self._rows(table, "table", i32, batch), self._vector(lens, "lens", batch),
-            self._vector(pos, "pos", batch), theta, m, p, track, sp, sb), "kq_kv_rope_attention")
+        hd = self.head_dim
+        heads = cols // hd - 2 * self.kv_heads
+        out_ld = self._rows(out, "out", f32, batch)
+        if (heads + 2 * self.kv_heads) * hd != cols or out.shape[1] < heads * hd:
+            raise _invalid(f"qkv rows of {cols} and out rows of {out.shape[1]} for heads of {hd}")
+        m, track = (None, 0) if mass is None else self._track(mass, "mass", f32, batch)
+        p = None
+        if slot_pos is not None:
+            p, track = self._track(slot_pos, "slot_pos", i32, batch, track)
+        rc = self._rope_attention(self.handle, qkv.data_ptr(), ld, out.data_ptr(), out_ld, batch, heads,
+                                  table.data_ptr(), self._rows(table, "table", i32, batch),
+                                  self._vector(lens, "lens", batch),
+                                  None if pos is None else self._vector(pos, "pos", batch), theta, m, p, track,
+                                  *self._scratch(scratch))
+        if rc:
+            self.ctx.check(rc, "kq_kv_rope_attention")
 
     def evict(self, table, lens, lens_out, mass, slot_pos, mass_out, pos_out, keep: int, scratch,
               recent_from=None) -> None:
@@ -193,7 +204,7 @@ class PagedCache:
         self.ctx.check(self.lib.kq_kv_evict(
             self.handle, batch, table.data_ptr(), self._rows(table, "table", i32), self._vector(lens, "lens", batch),
             self._vector(lens_out, "lens_out", batch), m, p, mo, po, track,
-            self._vector(recent_from, "recent_from", batch), keep, sp, sb), "kq_kv_evict")
+            None if recent_from is None else self._vector(recent_from, "recent_from", batch), keep, sp, sb), "kq_kv_evict")
 
     def close(self) -> None:
         if getattr(self, "handle", None):

@@ -23,25 +23,26 @@ def sample(ctx: "kq.Context", logits, u, tokens, *, temperature=None, top_k=None
     without a finite or +inf logit gives -1.  CUDA tensors on the context's
     device; queued on its stream."""
     import torch
-    dev = torch.device("cuda", ctx.device)
-    if logits.dtype != torch.float32 or logits.device != dev or logits.dim() != 2 or (
-            logits.shape[1] > 1 and logits.stride(1) != 1):
-        raise kq.KqError(kq.KQ_ERR_INVALID_ARG, f"logits: {logits.dtype} {tuple(logits.shape)} strides "
-                         f"{logits.stride()} on {logits.device}; rows of float32 on {dev} are wanted")
-    batch, vocab = logits.shape
+    f32, i32, index = torch.float32, torch.int32, ctx.device
+    shape, stride = logits.shape, logits.stride()
+    if logits.dtype is not f32 or logits.get_device() != index or len(shape) != 2 or (stride[1] != 1 and shape[1] > 1):
+        raise kq.KqError(kq.KQ_ERR_INVALID_ARG, f"logits: {logits.dtype} {tuple(shape)} strides {stride} on "
+                         f"{logits.device}; rows of float32 on cuda:{index} are wanted")
+    batch, vocab = shape
+    want = (batch,)
 
     def ptr(t, name, dtype):
         if t is None:
             return None
-        if t.dtype != dtype or t.device != dev or t.dim() != 1 or t.shape[0] != batch or (
-                batch > 1 and t.stride(0) != 1):
+        if t.dtype is not dtype or t.get_device() != index or t.shape != want or not t.is_contiguous():
             raise kq.KqError(kq.KQ_ERR_INVALID_ARG, f"{name}: {t.dtype} {tuple(t.shape)} on {t.device}; {batch} "
-                             f"contiguous {dtype} on {dev} are wanted")
+                             f"contiguous {dtype} on cuda:{index} are wanted")
         return t.data_ptr()
 
-    f32, i32 = torch.float32, torch.int32
-    ctx.check(_bind(ctx.lib).kq_dec_sample(
-        ctx.handle, logits.data_ptr(), logits.stride(0) if batch > 1 else vocab, batch, vocab,
+    rc = _bind(ctx.lib).kq_dec_sample(
+        ctx.handle, logits.data_ptr(), stride[0] if batch > 1 else vocab, batch, vocab,
         ptr(temperature, "temperature", f32), ptr(top_k, "top_k", i32), ptr(top_p, "top_p", f32),
         ptr(min_p, "min_p", f32), ptr(u, "u", f32), ptr(tokens, "tokens", i32), ptr(prob, "prob", f32),
-        ptr(kept, "kept", i32)), "kq_dec_sample")
+        ptr(kept, "kept", i32))
+    if rc:
+        ctx.check(rc, "kq_dec_sample")
