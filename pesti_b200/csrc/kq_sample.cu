@@ -55,11 +55,23 @@ __device__ __forceinline__ u64 word_of(float z, int i) { return (u64)order_key(z
 __device__ __forceinline__ float word_logit(u64 w) { return key_logit((uint32_t)(w >> 32)); }
 __device__ __forceinline__ int word_index(u64 w) { return (int)~(uint32_t)w; }
 
-// The last token that stays: those before it in the order do too.
+// The last token that stays: those before it in the order do too.  A token stays
+// where its logit is at least `z` (up to index i) or `above`, the next number (from
+// there on): one comparison each, the choice for four neighbours at once.
 struct Cut {
-  float z;
+  float z, above;
   int i;
-  __device__ __forceinline__ bool keeps(float f, int at) const { return f > z || (f == z && at <= i); }
+  __device__ __forceinline__ Cut(float z_, int i_) : z(z_), above(nextafterf(z_, INFINITY)), i(i_) {}
+  __device__ __forceinline__ bool keeps(float f, int at) const { return f >= (at <= i ? z : above); }
+  __device__ __forceinline__ void keeps4(const float (&f)[4], int at, bool (&stay)[4]) const {
+    const float least = at + 3 <= i ? z : above;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) stay[q] = f[q] >= least;
+    if ((unsigned)(i - at) < 3u) {  // the border lies among the four
+#pragma unroll
+      for (int q = 0; q < 4; ++q) stay[q] = keeps(f[q], at + q);
+    }
+  }
 };
 
 struct SampleShared {
@@ -74,6 +86,11 @@ struct SampleShared {
   u64 list[SM_LIST], weight[SM_LIST];  // first CTA: candidates
 };
 static_assert(sizeof(SampleShared) % 16 == 0, "the slice follows");
+// The CTA's shared memory: this, then its slice of the logits, padded with -inf.
+// (Named where it is used, so that every access is known to be one to shared memory.)
+extern __shared__ __align__(16) uint8_t sample_smem[];
+__device__ __forceinline__ SampleShared& shared() { return *reinterpret_cast<SampleShared*>(sample_smem); }
+__device__ __forceinline__ float* slice_logits() { return reinterpret_cast<float*>(sample_smem + sizeof(SampleShared)); }
 
 // Exclusive sum over the block's NT threads; `total` gets the sum.
 template <int NT>
@@ -156,16 +173,14 @@ struct Weights {
 template <int NT>
 struct Row {
   cg::cluster_group cluster;
-  SampleShared& S;
-  float* z;  // padded with -inf to whole quads
   int CL, rank, i0, n;
-  int turn = 0;  // the set of S.tot published last
+  int turn = 0;  // the set of shared().tot published last
 
   // f(z[4], first index) over the slice, four consecutive tokens at a time
   template <class F>
   __device__ __forceinline__ void each4(F f) {
     for (int i = 4 * threadIdx.x; i < n; i += 4 * NT) {
-      const float4 v = *reinterpret_cast<const float4*>(z + i);
+      const float4 v = *reinterpret_cast<const float4*>(slice_logits() + i);
       const float a[4] = {v.x, v.y, v.z, v.w};
       f(a, i0 + i);
     }
@@ -176,37 +191,36 @@ struct Row {
   __device__ __forceinline__ void publish(u64 a, u64 b) {
     turn ^= 1;
     if (threadIdx.x < CL) {
-      SampleShared* to = cluster.map_shared_rank(&S, threadIdx.x);
+      SampleShared* to = cluster.map_shared_rank(&shared(), threadIdx.x);
       to->tot[turn][rank] = a;
       to->tot2[turn][rank] = b;
     }
     cluster.sync();
   }
-  __device__ __forceinline__ u64 tot(int r) const { return S.tot[turn][r]; }
-  __device__ __forceinline__ u64 tot2(int r) const { return S.tot2[turn][r]; }
+  __device__ __forceinline__ u64 tot(int r) const { return shared().tot[turn][r]; }
+  __device__ __forceinline__ u64 tot2(int r) const { return shared().tot2[turn][r]; }
 
-  // The bins filled with measure(z) over bin_of(z, index) (-1: left out).
-  template <class Bin, class Measure>
-  __device__ void fill_bins(Bin bin_of, Measure measure) {
-    for (int e = threadIdx.x; e < SM_BINS; e += NT) S.lo[e] = S.hi[e] = 0;
+  // The bins filled with measure(z): bins_of(z[4], first index, bins[4]) says where
+  // (-1: left out).
+  template <class Bins, class Measure>
+  __device__ void fill_bins(Bins bins_of, Measure measure) {
+    for (int e = threadIdx.x; e < SM_BINS; e += NT) shared().lo[e] = shared().hi[e] = 0;
     __syncthreads();
     each4([&](const float (&v)[4], int i) {
       int k[4];
       u64 m[4];
       uint32_t old[4];
+      bins_of(v, i, k);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        k[q] = bin_of(v[q], i + q);
-        m[q] = measure(v[q]);
-      }
+      for (int q = 0; q < 4; ++q) m[q] = measure(v[q]);
 #pragma unroll
       for (int q = 0; q < 4; ++q)
-        if (k[q] >= 0) old[q] = atomicAdd(&S.lo[k[q]], (uint32_t)m[q]);
+        if (k[q] >= 0) old[q] = atomicAdd(&shared().lo[k[q]], (uint32_t)m[q]);
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         if (k[q] < 0) continue;
         const uint32_t h = (uint32_t)(m[q] >> 32) + (old[q] + (uint32_t)m[q] < old[q]);  // the carry
-        if (h) atomicAdd(&S.hi[k[q]], h);
+        if (h) atomicAdd(&shared().hi[k[q]], h);
       }
     });
   }
@@ -228,7 +242,7 @@ struct Row {
         uint32_t lo[SM_MAX_CLUSTER], hi[SM_MAX_CLUSTER];
 #pragma unroll
         for (int r = 0; r < SM_MAX_CLUSTER; ++r) {
-          const SampleShared* from = cluster.map_shared_rank(&S, r < CL ? r : 0);
+          const SampleShared* from = cluster.map_shared_rank(&shared(), r < CL ? r : 0);
           lo[r] = r < CL ? from->lo[rank * bins + e] : 0;
           hi[r] = r < CL ? from->hi[rank * bins + e] : 0;
         }
@@ -238,7 +252,7 @@ struct Row {
       sum += m[q];
     }
     u64 total;
-    u64 before = block_scan<NT>(sum, S.sums, total);
+    u64 before = block_scan<NT>(sum, shared().sums, total);
     publish(total, 0);
     u64 all = 0, start = 0;
     for (int r = 0; r < CL; ++r) {
@@ -251,15 +265,15 @@ struct Row {
 #pragma unroll
     for (int q = 0; q < MOST; ++q) {
       if (target > before && target <= before + m[q]) {
-        S.res[0] = (u64)(rank * bins + threadIdx.x * per + q);
-        S.res[1] = target - before;
+        shared().res[0] = (u64)(rank * bins + threadIdx.x * per + q);
+        shared().res[1] = target - before;
       }
       before += m[q];
     }
     int owner = 0;
     for (u64 sofar = tot(0); sofar < target; sofar += tot(owner)) ++owner;
     cluster.sync();
-    const SampleShared* from = cluster.map_shared_rank(&S, owner);
+    const SampleShared* from = cluster.map_shared_rank(&shared(), owner);
     bin = (int)from->res[0];
     left = from->res[1];
     return true;
@@ -270,7 +284,7 @@ struct Row {
   // CTA ends.
   template <class Pred>
   __device__ unsigned gather(Pred pred) {
-    SampleShared* first = cluster.map_shared_rank(&S, 0);
+    SampleShared* first = cluster.map_shared_rank(&shared(), 0);
     each4([&](const float (&v)[4], int i) {
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
@@ -290,19 +304,19 @@ struct Row {
     const unsigned listed = gather(pred);
     if (listed <= SM_LIST) {
       if (rank == 0) {
-        for (unsigned e = threadIdx.x; e < listed; e += NT) S.weight[e] = measure(word_logit(S.list[e]));
+        for (unsigned e = threadIdx.x; e < listed; e += NT) shared().weight[e] = measure(word_logit(shared().list[e]));
         __syncthreads();
         for (unsigned e = threadIdx.x; e < listed; e += NT) {
-          const u64 w = S.list[e];
+          const u64 w = shared().list[e];
           u64 before = 0;
-          for (unsigned j = 0; j < listed; ++j) before += S.list[j] > w ? S.weight[j] : 0;
-          if (before < left && left <= before + S.weight[e]) S.res[2] = w;
+          for (unsigned j = 0; j < listed; ++j) before += shared().list[j] > w ? shared().weight[j] : 0;
+          if (before < left && left <= before + shared().weight[e]) shared().res[2] = w;
         }
       }
       cluster.sync();
-      const u64 w = cluster.map_shared_rank(&S, 0)->res[2];
-      if (rank == 0 && threadIdx.x == 0) S.listed = 0;
-      return Cut{word_logit(w), word_index(w)};
+      const u64 w = cluster.map_shared_rank(&shared(), 0)->res[2];
+      if (rank == 0 && threadIdx.x == 0) shared().listed = 0;
+      return Cut(word_logit(w), word_index(w));
     }
     const Refined r = refine(*this, measure, left, pred);
     turn = r.turn;
@@ -338,16 +352,16 @@ struct Row {
     }
     __syncthreads();
     if ((threadIdx.x & 31) == 0) {
-      S.list[threadIdx.x >> 5] = low;
-      S.weight[threadIdx.x >> 5] = high;
+      shared().list[threadIdx.x >> 5] = low;
+      shared().weight[threadIdx.x >> 5] = high;
     }
     __syncthreads();
     for (int w = 0; w < NT / 32; ++w) {
-      low = S.list[w] < low ? S.list[w] : low;
-      high = S.weight[w] > high ? S.weight[w] : high;
+      low = shared().list[w] < low ? shared().list[w] : low;
+      high = shared().weight[w] > high ? shared().weight[w] : high;
     }
     publish(low, high);
-    if (rank == 0 && threadIdx.x == 0) S.listed = 0;
+    if (rank == 0 && threadIdx.x == 0) shared().listed = 0;
     for (int r = 0; r < CL; ++r) {
       low = tot(r) < low ? tot(r) : low;
       high = tot2(r) > high ? tot2(r) : high;
@@ -357,9 +371,12 @@ struct Row {
       int bin = 0;
       const u64 goal = left;
       fill_bins(
-          [&](float f, int i) {
-            const u64 w = word_of(f, i);
-            return w >= low && w <= high && pred(f, i) ? SM_BINS - 1 - (int)((w - low) >> shift) : -1;
+          [&](const float (&v)[4], int i, int (&k)[4]) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const u64 w = word_of(v[q], i + q);
+              k[q] = w >= low && w <= high && pred(v[q], i + q) ? SM_BINS - 1 - (int)((w - low) >> shift) : -1;
+            }
           },
           measure);
       find_bin([&](u64) { return goal; }, bin, left);
@@ -367,15 +384,16 @@ struct Row {
       const u64 top = low + ((1ull << shift) - 1);
       high = top < high ? top : high;
     }
-    return Refined{Cut{word_logit(low), word_index(low)}, turn};
+    return Refined{Cut(word_logit(low), word_index(low)), turn};
   }
 };
 
 // What a row's first CTA does alone: `m` candidates in S.list hold the first K <=
 // NT tokens; top-p, min-p (logits from `least` up) and the draw among those.
 template <int NT, class Answer>
-__device__ __noinline__ void draw_from_list(SampleShared& S, Weights W, int m, int K, double P, float least, double U,
+__device__ __noinline__ void draw_from_list(Weights W, int m, int K, double P, float least, double U,
                                             Answer answer) {
+  SampleShared& S = shared();
   const int tid = threadIdx.x;
   for (int e = tid; e < m; e += NT) {  // into their order
     const u64 w = S.list[e];
@@ -405,15 +423,14 @@ __device__ __noinline__ void draw_from_list(SampleShared& S, Weights W, int m, i
 // NT 512: two CTAs per SM; 1024: one
 template <int NT>
 __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs A, int slice, int frac) {
-  extern __shared__ __align__(16) uint8_t dyn[];
-  SampleShared& S = *reinterpret_cast<SampleShared*>(dyn);
+  SampleShared& S = shared();
   cg::cluster_group cluster = cg::this_cluster();
   const int CL = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int64_t b = blockIdx.x / CL;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int i0 = min(A.vocab, rank * slice), n = min(A.vocab, i0 + slice) - i0;  // this CTA's tokens
-  float* z = reinterpret_cast<float*>(dyn + sizeof(SampleShared));
-  Row<NT> R{cluster, S, z, CL, rank, i0, n};
+  float* z = slice_logits();
+  Row<NT> R{cluster, CL, rank, i0, n};
   cluster.barrier_arrive();  // this CTA has started
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (tid < 16) {  // 2^(i / 256) = 2^(16 a / 256) 2^(b / 256)
@@ -421,7 +438,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
     if (tid) S.pow2[tid] = exp2(frac + tid / 256.0);
   }
   if (tid == 0) S.listed = 0;
-  if (tid < 4) z[n + tid] = -INFINITY;
+  if (tid < 8) z[n + tid] = -INFINITY;
   for (int e = tid; e < SM_BINS; e += NT) S.lo[e] = 0;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   // the slice into shared memory, 16 bytes a copy where the row allows it
@@ -527,13 +544,13 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
   auto fixed = [W](float f) { return W.fixed(f); };
   auto one = [](float) { return (u64)1; };
 
-  Cut cut{-INFINITY, -1};
+  Cut cut(-INFINITY, -1);
   if (K > 0) {
     if (kth > -INFINITY && !endless) {
       const unsigned listed = R.gather([&](float f, int) { return f >= kth; });
       cluster.sync();
       if (listed <= SM_LIST) {
-        if (rank == 0) draw_from_list<NT>(S, W, (int)listed, K, P, least, U, answer);
+        if (rank == 0) draw_from_list<NT>(W, (int)listed, K, P, least, U, answer);
         return;
       }
       if (rank == 0 && tid == 0) S.listed = 0;
@@ -545,7 +562,12 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
     };
     int bin = 0;
     u64 left = 0;
-    R.fill_bins([&](float f, int) { return near(f); }, one);
+    R.fill_bins(
+        [&](const float (&v)[4], int, int (&k)[4]) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) k[q] = near(v[q]);
+        },
+        one);
     if (R.find_bin([&](u64) { return (u64)K; }, bin, left)) {
       cut = R.border(one, left, [near, bin](float f, int) { return near(f) == bin; });
     } else {
@@ -565,27 +587,32 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
     int bin = 0;
     u64 left = 0;
     const Cut first_k = cut;
-    R.fill_bins([&](float f, int i) { return first_k.keeps(f, i) ? W.bin(f) : -1; }, fixed);
+    R.fill_bins(
+        [&](const float (&v)[4], int i, int (&k)[4]) {
+          bool stay[4];
+          first_k.keeps4(v, i, stay);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) k[q] = stay[q] ? W.bin(v[q]) : -1;
+        },
+        fixed);
     R.find_bin([&](u64 all) { return min(max((u64)ceil(P * (double)all), 1ull), all); }, bin, left);
     cut = R.border(fixed, left, [W, bin, first_k](float f, int i) { return W.bin(f) == bin && first_k.keeps(f, i); });
   }
 
-  if (least > cut.z) cut = Cut{least, INT_MAX};
+  if (least > cut.z) cut = Cut(least, INT_MAX);
 
-  // ---- the draw: thread t sums tokens [t c, (t + 1) c) of the slice (c odd: no bank is hit twice) ----
-  const int c = ((n + NT - 1) / NT) | 1;
-  const int t0 = min(n, tid * c), t1 = min(n, t0 + c);
+  // ---- the draw: thread t sums the quads [t c, (t + 1) c) of the slice (c odd: no bank is hit twice) ----
+  const int quads_here = (n + 3) / 4, c = ((quads_here + NT - 1) / NT) | 1;
+  const int t0 = 4 * min(quads_here, tid * c), t1 = 4 * min(quads_here, tid * c + c);
   u64 sum = 0;
   unsigned count = 0;
-  for (int j = 0; j < c; j += 4) {
-    float f[4];
+  for (int j = 0; j < c; ++j) {
+    const int i = min(t0 + 4 * j, t1);  // (past the thread's quads: one of the next, or the padding, left out)
+    const float4 v = *reinterpret_cast<const float4*>(z + i);
+    const float f[4] = {v.x, v.y, v.z, v.w};
     bool stay[4];
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int i = t0 + j + q;
-      f[q] = z[min(i, n)];
-      stay[q] = i < t1 && cut.keeps(f[q], i0 + i);
-    }
+    cut.keeps4(f, i0 + i, stay);
+    if (i >= t1) stay[0] = stay[1] = stay[2] = stay[3] = false;
     if (!__any_sync(0xffffffffu, stay[0] || stay[1] || stay[2] || stay[3])) continue;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
@@ -620,12 +647,12 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
   }
 }
 
-size_t sample_smem(int slice) { return sizeof(SampleShared) + ((size_t)slice + 4) * sizeof(float); }
+size_t sample_bytes(int slice) { return sizeof(SampleShared) + ((size_t)slice + 8) * sizeof(float); }
 
 }  // namespace
 
 cudaError_t sample_init_device() {
-  const int most = (int)sample_smem(SM_SLICE);
+  const int most = (int)sample_bytes(SM_SLICE);
   cudaError_t e = cudaFuncSetAttribute(sample_kernel<512>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
   if (e == cudaSuccess)
     e = cudaFuncSetAttribute(sample_kernel<1024>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
@@ -651,7 +678,7 @@ cudaError_t dec_sample(const SampleArgs& a, int num_sms, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.batch * cl));
   cfg.blockDim = dim3(wide ? 1024 : 512);
-  cfg.dynamicSmemBytes = sample_smem(slice);
+  cfg.dynamicSmemBytes = sample_bytes(slice);
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
