@@ -1304,7 +1304,8 @@ int kq_kv_create(kq_ctx* ctx, void* k_pool, void* v_pool, int64_t pages, int64_t
   kv->pool.page_size = page_size;
   kv->pool.hkv = kv_heads;
   kv->pool.hd = head_dim;
-  if (!kq::kv_make_maps(kv->pool, &kv->maps)) {
+  DeviceGuard g(ctx->device);
+  if (g.status != cudaSuccess || !kq::kv_make_maps(kv->pool, &kv->maps)) {
     delete kv;
     return fail(ctx, KQ_ERR_CUDA, "kq_kv_create: the driver refused the pools' TMA descriptors");
   }
@@ -1327,8 +1328,10 @@ static int kv_check(kq_kv* kv, const char* what, const int32_t* table, int64_t t
   return KQ_OK;
 }
 
-static int kv_heads_check(kq_kv* kv, const char* what, int heads) {
+static int kv_heads_check(kq_kv* kv, const char* what, int heads, int64_t batch) {
   const int hkv = kv->pool.hkv;
+  if (batch * heads > INT32_MAX)
+    return fail(kv->ctx, KQ_ERR_INVALID_ARG, "%s: %lld sequences of %d query heads", what, (long long)batch, heads);
   if (heads < hkv || heads % hkv || heads / hkv > kq::KV_MAX_GROUP)
     return fail(kv->ctx, KQ_ERR_UNSUPPORTED, "%s: %d query heads over %d kv heads (1 to %d per kv head)", what, heads,
                 hkv, kq::KV_MAX_GROUP);
@@ -1345,10 +1348,10 @@ int kq_kv_append(kq_kv* kv, const float* qkv, int64_t ld, int64_t rows, int head
   const char* what = "kq_kv_append";
   if (rows > 0 && (!qkv || !slots)) return fail(ctx, KQ_ERR_INVALID_ARG, "%s: null qkv or slots", what);
   if (int rc = kv_check(kv, what, table, table_ld, batch)) return rc;
-  if (int rc = kv_heads_check(kv, what, heads)) return rc;
+  if (int rc = kv_heads_check(kv, what, heads, batch)) return rc;
   const int64_t hd = kv->pool.hd;
   if (rows < 0 || rows > INT32_MAX || ld < (heads + 2 * (int64_t)kv->pool.hkv) * hd || (q_out && q_ld < heads * hd) ||
-      (slot_pos && track_ld < 1) || (!seqs && rows > batch) || bad_theta(theta))
+      (q_out == qkv && q_ld != ld && rows > 1) || (slot_pos && track_ld < 1) || (!seqs && rows > batch) || bad_theta(theta))
     return fail(ctx, KQ_ERR_INVALID_ARG, "%s: %lld rows of %lld, q rows of %lld, theta %g", what, (long long)rows,
                 (long long)ld, (long long)q_ld, (double)theta);
   if (rows == 0) return KQ_OK;
@@ -1379,7 +1382,7 @@ int kq_kv_append(kq_kv* kv, const float* qkv, int64_t ld, int64_t rows, int head
 
 size_t kq_kv_attention_scratch(const kq_kv* kv, int64_t batch, int heads, int64_t track_len) {
   if (!kv || batch < 1 || batch > 65535 || heads < kv->pool.hkv || heads % kv->pool.hkv ||
-      heads / kv->pool.hkv > kq::KV_MAX_GROUP || track_len < 0)
+      heads / kv->pool.hkv > kq::KV_MAX_GROUP || batch * heads > INT32_MAX || track_len < 0 || track_len > INT32_MAX)
     return 0;
   return kq::kv_attention_scratch_bytes(batch, heads, kv->pool.hkv, kv->pool.hd, track_len, kv->ctx->num_sms);
 }
@@ -1392,7 +1395,7 @@ static int kv_attention_impl(kq_kv* kv, const char* what, bool rope, const float
   kq_ctx* ctx = kv->ctx;
   if (!q || !out || !lens || !scratch) return fail(ctx, KQ_ERR_INVALID_ARG, "%s: null argument", what);
   if (int rc = kv_check(kv, what, table, table_ld, batch)) return rc;
-  if (int rc = kv_heads_check(kv, what, heads)) return rc;
+  if (int rc = kv_heads_check(kv, what, heads, batch)) return rc;
   const int64_t hd = kv->pool.hd, cols = (rope ? heads + 2 * (int64_t)kv->pool.hkv : heads) * hd;
   if (q_ld < cols || out_ld < heads * hd || ((mass || slot_pos) && (track_ld < 1 || track_ld > INT32_MAX)) ||
       (rope && bad_theta(theta)))

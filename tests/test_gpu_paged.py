@@ -411,7 +411,8 @@ def test_append_in_place_and_defaults(gpu_ctx):
     c1 = paged.PagedCache(gpu_ctx, k1, v1)
     torch.cuda.synchronize()
     c1.append(qkv, s.table, slots, theta=1e4)
-    s.cache.append(qkv, s.table, slots, theta=1e4, q_out=qkv)
+    s.cache.append(qkv[:1], s.table, slots[:1], theta=1e4, q_out=qkv[:1, :hq * hd])
+    s.cache.append(qkv[1:], s.table[1:], slots[1:], theta=1e4, q_out=qkv[1:])
     gpu_ctx.synchronize()
     assert float((qkv[:, :hq * hd].view(3, hq, hd).double() - want).abs().max()) <= TOL_TURN * float(want.abs().max()) * 2
     assert torch.equal(qkv[:, hq * hd:], rest)
@@ -571,6 +572,9 @@ def test_pools_and_sizes_that_are_refused(gpu_ctx):
         assert status(c.rope_attention, qkv, table, lens, out, scratch, theta=theta) == bad
         assert status(c.append, qkv, table, lens, theta=theta) == bad
     assert status(c.append, torch.zeros((2, 6 * 64), **f), table, torch.zeros(2, **i), theta=1e4) == bad
+    two = torch.zeros((2, 6 * 64), **f)  # q_out over qkv at another stride
+    assert status(c.append, two, table, torch.zeros(2, **i), theta=1e4, seqs=torch.zeros(2, **i),
+                  q_out=two.as_strided((2, 128), (128, 1))) == bad
     m, p = torch.zeros((1, 2, 32), **f), torch.zeros((1, 2, 32), **i)
     es = c.evict_scratch(1, 32)
     assert status(c.evict, table, lens, lens, m, p, m, p, 0, es) == bad
