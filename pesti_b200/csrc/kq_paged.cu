@@ -129,7 +129,9 @@ __global__ void __launch_bounds__(AP_THREADS, 8) kv_append_kernel(const KvAppend
 // consecutive slots as bits of a mask.  Keys are read from global memory once and
 // stay in shared memory (up to EV_PIECE slots a CTA; longer shares go piece by
 // piece).  A second kernel moves the rows: it is bound by them, the first by the
-// latency of its passes.
+// latency of its passes.  Measured: 8 sequences of 2113 to 2048 slots, 8 heads of 128,
+// 13.8 us; 4 of up to 32,771 to 4096 30.9 us, of which the rows take about half (33 MB
+// read, as much written).
 constexpr int EV_THREADS = 512, EV_BINS = 2048, EV_PIECE = 20480, EV_LOADS = 8, EV_MAX_CLUSTER = 8;
 constexpr size_t EV_SMEM = (size_t)EV_PIECE * 4;
 
