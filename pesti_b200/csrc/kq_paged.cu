@@ -68,8 +68,8 @@ __global__ void __launch_bounds__(AP_THREADS, 8) kv_append_kernel(const KvAppend
   load(first + tid);
   const int32_t slot = r < A.rows ? A.slots[r] : -1;
   const int64_t b = slot >= 0 && A.seqs ? A.seqs[r] : r;
-  const bool bad = slot >= 0 && (b < 0 || b >= A.batch || slot >= A.table_ld * A.pool.page_size ||
-                                 (A.slot_pos && slot >= A.track_ld));
+  const bool bad = slot < -1 || (slot >= 0 && (b < 0 || b >= A.batch || slot >= A.table_ld * A.pool.page_size ||
+                                               (A.slot_pos && slot >= A.track_ld)));
   if (bad && tid == 0) kv_error(A.err, KV_ERR_ROW);
   const bool live = slot >= 0 && !bad;
   int32_t pos = 0;
@@ -222,7 +222,7 @@ __global__ void __launch_bounds__(EV_THREADS, 2) kv_evict_select_kernel(const Kv
   };
   if (len <= keep) {
     each(stays_put);
-    if (part == 0 && tid == 0) *plan = EvictPlan{0, new_len, {0, 0}};
+    if (part == 0 && tid == 0) *plan = EvictPlan{0, bad ? A.lens[b] : new_len, {0, 0}};
     return;
   }
   auto sync_all = [&] {

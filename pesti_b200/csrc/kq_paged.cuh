@@ -12,10 +12,11 @@ namespace kq {
 // Device error codes of the paged cache and its callers (the context's error word).
 enum : int { KV_ERR_PAGE = 51, KV_ERR_LEN = 52, KV_ERR_ROW = 53, KV_ERR_WAIT = 54 };
 
-// A sequence's slots in use: lens[b] held to [0, most]; *bad is set where it was outside.
+// A sequence's slots in use; where lens[b] is outside [0, most], *bad is set and the
+// sequence counts as idle (held to `most`, a step would overwrite its last slot).
 __host__ __device__ __forceinline__ int64_t kv_len(int32_t len, int64_t most, bool* bad) {
   *bad = len < 0 || len > most;
-  return len < 0 ? 0 : len > most ? most : (int64_t)len;
+  return *bad ? 0 : (int64_t)len;
 }
 
 // Element offset of slot's row for one kv head, or -1 where the table's page

@@ -145,7 +145,7 @@ __device__ __forceinline__ void tma_load_5d(void* dst, const CUtensorMap* map, i
       : "memory");
 }
 
-// Slots a sequence uses, held to its block table (and to the tracked slots).
+// Slots a sequence uses: none where its block table (or the tracked slots) cannot hold them.
 __device__ __forceinline__ int pa_len(const KvAttnArgs& A, int64_t b, bool* bad) {
   int64_t most = A.table_ld * A.pool.page_size;
   if (A.mass || A.slot_pos) most = min(most, A.track_ld);

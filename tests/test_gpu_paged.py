@@ -585,7 +585,31 @@ def test_pools_and_sizes_that_are_refused(gpu_ctx):
     assert gpu_ctx.launch_count == before  # no rows: nothing is queued
 
 
-@pytest.mark.parametrize("what", ["page", "negative", "far page", "len", "negative len", "slot", "seq"])
+def test_a_length_past_the_table_leaves_the_cache_alone(gpu_ctx):
+    """A sequence that outgrew its table is an idle row: its last slot is not overwritten,
+    evicting it changes neither its length nor its rows."""
+    hd, hkv, page = 64, 2, 16
+    s = Setup(gpu_ctx, [48, 20], 2, hkv, hd, page, seed=2)
+    table = s.table[:, :3].clamp(0, s.pages - 1).contiguous()
+    lens = torch.tensor([49, 21], dtype=torch.int32, device=DEV)
+    qkv, out = torch.randn((2, 6 * hd), device=DEV), torch.full((2, 2 * hd), 7.0, device=DEV)
+    m, p = torch.rand((2, hkv, 48), device=DEV), torch.arange(48, dtype=torch.int32, device=DEV).expand(2, hkv, 48).contiguous()
+    scratch, es = s.cache.scratch(2, 2, 48), s.cache.evict_scratch(2, 48)
+    rows = [s.k[s.table[0, j // page].long(), :, j % page].clone() for j in range(48)]
+    m0, p0 = m.clone(), p.clone()
+    torch.cuda.synchronize()
+    s.cache.rope_attention(qkv, table, lens, out, scratch, theta=1e4, mass=m, slot_pos=p)
+    assert status(gpu_ctx.synchronize) == kq.KQ_ERR_INVALID_ARG
+    s.cache.evict(table, lens, lens, m, p, m, p, 30, es)
+    assert status(gpu_ctx.synchronize) == kq.KQ_ERR_INVALID_ARG
+    assert lens.tolist() == [49, 21]
+    assert torch.equal(out[0], torch.zeros_like(out[0])) and out[1].isfinite().all() and bool(out[1].abs().max() > 0)
+    assert torch.equal(m[0], m0[0]) and torch.equal(p[0], p0[0])
+    for j in range(48):
+        assert torch.equal(s.k[s.table[0, j // page].long(), :, j % page], rows[j])
+
+
+@pytest.mark.parametrize("what", ["page", "negative", "far page", "len", "negative len", "slot", "far slot", "seq"])
 def test_what_lies_outside_is_reported_and_not_followed(gpu_ctx, what):
     hd, hkv, page = 64, 2, 16
     s = Setup(gpu_ctx, [40, 20], 2, hkv, hd, page, seed=1)
@@ -600,10 +624,10 @@ def test_what_lies_outside_is_reported_and_not_followed(gpu_ctx, what):
     scratch, es = s.cache.scratch(2, 2, 48), s.cache.evict_scratch(2, 48)
     k0 = s.k.clone()
     torch.cuda.synchronize()
-    if what in ("slot", "seq"):
+    if what in ("slot", "far slot", "seq"):
         qkv = torch.randn((2, 6 * hd), device=DEV)
-        slots = torch.tensor([48 if what == "slot" else 3, -1], dtype=torch.int32, device=DEV)
-        seqs = torch.tensor([0 if what == "slot" else 2, 0], dtype=torch.int32, device=DEV)
+        slots = torch.tensor([{"slot": 48, "far slot": -2, "seq": 3}[what], -1], dtype=torch.int32, device=DEV)
+        seqs = torch.tensor([2 if what == "seq" else 0, 0], dtype=torch.int32, device=DEV)
         table = table[:, :3].contiguous()
         torch.cuda.synchronize()
         s.cache.append(qkv, table, slots, theta=1e4, seqs=seqs)

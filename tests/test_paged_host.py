@@ -82,7 +82,7 @@ int main() {
   bool bad;
   CHECK(kv_len(0, 100, &bad) == 0 && !bad);
   CHECK(kv_len(100, 100, &bad) == 100 && !bad);
-  CHECK(kv_len(101, 100, &bad) == 100 && bad);
+  CHECK(kv_len(101, 100, &bad) == 0 && bad);
   CHECK(kv_len(-1, 100, &bad) == 0 && bad);
   CHECK(kv_len(0x7fffffff, 1ll << 40, &bad) == 0x7fffffff && !bad);
   const int sizes[][2] = {{16, 16}, {32, 32}, {48, 16}, {64, 64}, {96, 32}, {128, 64}, {1024, 64}, {1008, 16}};
