@@ -77,8 +77,12 @@ __global__ void __launch_bounds__(AP_THREADS, 8) kv_append_kernel(const KvAppend
   if (live) {
     const int32_t page = A.table[b * A.table_ld + slot / A.pool.page_size];
     pos = A.pos ? A.pos[r] : slot;
-    for (int i = tid; i < half; i += TPR)
-      rope_turn(pos, freq[i], reinterpret_cast<float*>(turn_c)[i], reinterpret_cast<float*>(turn_s)[i]);
+    for (int i = tid; i < half; i += TPR) {
+      double c, s;
+      rope_turn(pos, freq[i], c, s);
+      reinterpret_cast<float*>(turn_c)[i] = (float)c;
+      reinterpret_cast<float*>(turn_s)[i] = (float)s;
+    }
     row0 = kv_row(A.pool, page, slot, 0);
     if (row0 < 0 && tid == 0) kv_error(A.err, KV_ERR_PAGE);
   }

@@ -38,12 +38,20 @@ __device__ __forceinline__ void kv_error(int* err, int code) { atomicCAS(err, 0,
 __device__ __forceinline__ double rope_freq(int i, int half, double log2_theta) {
   return exp2(-(double)i / (double)half * log2_theta) * 0.15915494309189533577;
 }
-// cos / sin of pos * theta^(-i / half).  The angle is reduced in 64 bits: at
-// position 100,000 an f32 angle is off by 4e-3, where the f32 result of this
-// form stays within 1e-7 of the exact one.
-__device__ __forceinline__ void rope_turn(int32_t pos, double freq, float& c, float& s) {
-  const double t = (double)pos * freq;
-  sincospif(2.f * (float)(t - rint(t)), &s, &c);
+// cos / sin of pos * theta^(-i / half), in 64 bits: at position 100,000 an f32 angle
+// is off by 4e-3.  To the nearest quarter turn, then the power series at |r| <= pi / 4,
+// whose first terms left out are r^13 / 13! < 7e-12 and r^14 / 14! < 4e-13.
+__device__ __forceinline__ void rope_turn(int32_t pos, double freq, double& c, double& s) {
+  constexpr double F3 = 1.0 / 6, F5 = 1.0 / 120, F7 = 1.0 / 5040, F9 = 1.0 / 362880, F11 = 1.0 / 39916800;
+  constexpr double F4 = 1.0 / 24, F6 = 1.0 / 720, F8 = 1.0 / 40320, F10 = 1.0 / 3628800, F12 = 1.0 / 479001600;
+  const double t = 4.0 * ((double)pos * freq), n = rint(t);
+  const double r = (t - n) * 1.5707963267948966192, x = -r * r;
+  const double si = r * fma(x, fma(x, fma(x, fma(x, fma(x, F11, F9), F7), F5), F3), 1.0);
+  const double co = fma(x, fma(x, fma(x, fma(x, fma(x, fma(x, F12, F10), F8), F6), F4), 0.5), 1.0);
+  const int quarter = (int)(int64_t)n & 3;
+  const double a = quarter & 1 ? si : co, b = quarter & 1 ? co : si;
+  c = quarter == 1 || quarter == 2 ? -a : a;
+  s = quarter & 2 ? -b : b;
 }
 #endif
 

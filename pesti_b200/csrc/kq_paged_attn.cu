@@ -382,7 +382,7 @@ __global__ void __launch_bounds__(PaCfg<HD, NS>::THREADS, PaCfg<HD, NS>::CTAS)
       new_page = A.table[at.b * A.table_ld + (at.len - 1) / A.pool.page_size];
     }
   };
-  float cs[IN][2], sn[IN][2];
+  float cs[IN][2], sn[IN][2], cs_lo[IN][2], sn_lo[IN][2];  // cosines and sines, and what f32 leaves of them
 #pragma unroll
   for (int k = 0; k < IN; ++k) cs[k][0] = cs[k][1] = 1.f, sn[k][0] = sn[k][1] = 0.f;
   int64_t turned = -1;  // the sequence that cs, sn are for
@@ -401,7 +401,14 @@ __global__ void __launch_bounds__(PaCfg<HD, NS>::THREADS, PaCfg<HD, NS>::CTAS)
 #pragma unroll
         for (int k = 0; k < IN; ++k)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) rope_turn(pos, rope_freq(qi + 64 * k + e, HALF, A.log2_theta), cs[k][e], sn[k][e]);
+          for (int e = 0; e < 2; ++e) {
+            double co, si;
+            rope_turn(pos, rope_freq(qi + 64 * k + e, HALF, A.log2_theta), co, si);
+            cs[k][e] = (float)co;
+            sn[k][e] = (float)si;
+            cs_lo[k][e] = (float)(co - (double)cs[k][e]);
+            sn_lo[k][e] = (float)(si - (double)sn[k][e]);
+          }
         turned = W.b;
       }
 #pragma unroll
@@ -448,9 +455,17 @@ __global__ void __launch_bounds__(PaCfg<HD, NS>::THREADS, PaCfg<HD, NS>::CTAS)
         for (int k = 0; k < IN; ++k) {
           const int i = qi + 64 * k;
           __half2 a, b;
-          if (w == 0) {
-            a = __floats2half2_rn(nr[k][0] * cs[k][0] - nr[k][2] * sn[k][0], nr[k][1] * cs[k][1] - nr[k][3] * sn[k][1]);
-            b = __floats2half2_rn(nr[k][0] * sn[k][0] + nr[k][2] * cs[k][0], nr[k][1] * sn[k][1] + nr[k][3] * cs[k][1]);
+          if (w == 0) {  // in 64 bits to the nearest f32 (sums in f32 would round another way to f16 at 2e-4 of them)
+            float ab[2][2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const double co = (double)cs[k][e] + cs_lo[k][e], si = (double)sn[k][e] + sn_lo[k][e];
+              const double x = nr[k][e], y = nr[k][e + 2];
+              ab[0][e] = (float)(x * co - y * si);
+              ab[1][e] = (float)(x * si + y * co);
+            }
+            a = __floats2half2_rn(ab[0][0], ab[0][1]);
+            b = __floats2half2_rn(ab[1][0], ab[1][1]);
           } else {
             a = __floats2half2_rn(nr[k][0], nr[k][1]);
             b = __floats2half2_rn(nr[k][2], nr[k][3]);

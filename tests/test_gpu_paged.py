@@ -196,6 +196,23 @@ def test_rope_attention(gpu_ctx, hd, hq, hkv, page, lens):
         assert torch.equal(mass[b, h, n:], mass0[b, h, n:])
 
 
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_the_appended_key_is_the_exact_one_rounded(gpu_ctx, hd):
+    """k is turned in 64 bits, to 1e-10 of its length, rounded to f32 and that to f16 (as torch
+    converts a double): the first rounding moves at about 1e-3 of the elements, which moves the
+    second at 1e-4 of those, where sums in f32 would at 2e-4 of all."""
+    B, hq, hkv, theta = 64 * 256 // hd, 4, 4, 1e6
+    s = Setup(gpu_ctx, [3] * B, hq, hkv, hd, 16, seed=hd)
+    qkv = torch.randn((B, (hq + 2 * hkv) * hd), generator=s.g, device=DEV)
+    pos = torch.randint(0, 120000, (B,), generator=s.g, device=DEV).int()
+    out = torch.zeros((B, hq * hd), device=DEV)
+    torch.cuda.synchronize()
+    s.cache.rope_attention(qkv, s.table, s.lens, out, s.cache.scratch(B, hq, 0), theta=theta, pos=pos)
+    gpu_ctx.synchronize()
+    want = turn(qkv.view(B, hq + 2 * hkv, hd)[:, hq:hq + hkv], pos, theta).half()
+    assert int((s.k[s.table[:, 0].long(), :, 2] != want).sum()) <= 2  # of 65,536
+
+
 def test_default_positions_and_the_contiguous_cache_agree(gpu_ctx):
     """Pages in order are the contiguous cache: kq_dec_rope_attention's own result."""
     hd, hq, hkv, B, pos, page = 128, 32, 8, 3, 300, 16
