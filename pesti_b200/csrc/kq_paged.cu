@@ -20,8 +20,8 @@ namespace cg = cooperative_groups;
 // shared memory, then four consecutive pairs of a head per thread and step.  Bound
 // by the row's bytes: f32 in, f32 q and f16 k, v out.  Many small CTAs hide the chain
 // slot - page - row better than several steps' loads in flight: 4099 rows of 32 / 8
-// heads of 128 take 33.2 us with one step and eight CTAs per SM (5569 GB/s), 38.9
-// with four steps and four.
+// heads of 128 took 33.2 us with one step and eight CTAs per SM, 38.9 with four steps
+// and four (34.5 us, 5360 GB/s, since sines are 64-bit as well).
 constexpr int AP_THREADS = 256, AP_MAX_HALF = 128;
 
 // Four floats at p, in one access where `vec` (p is then 16-byte aligned).
