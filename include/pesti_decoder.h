@@ -179,7 +179,8 @@ int kq_step_destroy(kq_step *step);
  * queued on its stream.  lens, slots, positions and table entries are read on
  * the device, so a captured graph replays with their values of the moment.
  * One that lies outside its bounds is not followed: nothing is read or written
- * there, and the next kq_ctx_synchronize reports KQ_ERR_INVALID_ARG.  A length
+ * there, and the next kq_ctx_synchronize reports KQ_ERR_INVALID_ARG (the calls
+ * queued in between run as they would without it).  A length
  * that the table (or track_ld) cannot hold makes its sequence an idle row of
  * that call, which leaves its cache, mass and lens_out as lens had it.
  * No reference counterpart: its cache is one contiguous block per sequence

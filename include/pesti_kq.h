@@ -96,7 +96,9 @@ int kq_ctx_destroy(kq_ctx *ctx);
 /* Install an external cudaStream_t (NULL restores the context's own). */
 int kq_ctx_set_stream(kq_ctx *ctx, void *cuda_stream);
 /* Wait for the context stream; also reports a device-side pipeline error of
- * an earlier asynchronous call (KQ_ERR_CUDA with a message). */
+ * an earlier asynchronous call (KQ_ERR_CUDA with a message), as every synchronous
+ * call does, and what a paged-cache call met out of its bounds
+ * (KQ_ERR_INVALID_ARG, pesti_decoder.h), which this call alone reports. */
 int kq_ctx_synchronize(kq_ctx *ctx);
 /* Select the kernel family for GGUF weights (KQ_PATH_*). */
 int kq_ctx_set_path(kq_ctx *ctx, int path);

@@ -27,8 +27,12 @@ struct kq_ctx {
   size_t ws_bytes = 0;
   void* ctr = nullptr;  // split-K arrival counters: zero between calls
   size_t ctr_bytes = 0;
-  int* dev_err = nullptr;   // set by a tensor-core kernel whose pipeline wait gave up
+  // Two words: [0] a device-side wait that gave up (every bounded wait polls it and
+  // gives up too), [1] lengths, slots or pages out of their bounds, which concern the
+  // call that met them alone (nothing on the device reads it).
+  int* dev_err = nullptr;
   int* host_err = nullptr;  // pinned mirror of dev_err, read after synchronising
+  int* dev_bad() const { return dev_err + 1; }
   void* xbuf = nullptr;     // device staging of host inputs
   size_t xbuf_bytes = 0;
   void* ybuf = nullptr;  // device staging of host outputs
@@ -191,22 +195,14 @@ int check_ctx(kq_ctx* ctx) { return ctx ? KQ_OK : KQ_ERR_INVALID_ARG; }
 
 // After the stream is synchronised: report (and clear) a device-side wait
 // that gave up.  The split-K counters may then be stale, so they are cleared too.
-int check_device_error(kq_ctx* ctx) {
-  const int code = *reinterpret_cast<volatile int*>(ctx->host_err);
+int check_wait_error(kq_ctx* ctx) {
+  const int code = reinterpret_cast<volatile int*>(ctx->host_err)[0];
   if (code == 0) return KQ_OK;
-  *ctx->host_err = 0;
+  ctx->host_err[0] = 0;
   cudaMemset(ctx->dev_err, 0, sizeof(int));
   if (ctx->ctr) cudaMemset(ctx->ctr, 0, ctx->ctr_bytes);
   cudaDeviceSynchronize();
   cudaGetLastError();
-  if (code >= 51 && code <= 53)
-    return fail(ctx, KQ_ERR_INVALID_ARG,
-                "a paged-cache call met %s (code %d); nothing was read or written there and the call's output is "
-                "invalid",
-                code == 51   ? "a page outside the pool"
-                : code == 52 ? "a sequence length outside its block table"
-                             : "a row whose sequence or slot lies outside the block table",
-                code);
   return fail(ctx, KQ_ERR_CUDA,
               "a device-side wait gave up (code %d: 1-5 tcgen05 pipeline, 21-23 decode weight ring, "
               "27-28 batched integer-MMA ring, 31-32 tensor-parallel peer flag, 41-45 decode-step ring, "
@@ -214,16 +210,39 @@ int check_device_error(kq_ctx* ctx) {
               code);
 }
 
-// Stream-ordered copy of the device error word into the pinned mirror.
-cudaError_t stage_error_word(kq_ctx* ctx) {
-  return cudaMemcpyAsync(ctx->host_err, ctx->dev_err, sizeof(int), cudaMemcpyDeviceToHost, ctx->stream);
+// The same for what a paged-cache call met out of its bounds.
+int check_bad_input(kq_ctx* ctx) {
+  const int code = reinterpret_cast<volatile int*>(ctx->host_err)[1];
+  if (code == 0) return KQ_OK;
+  ctx->host_err[1] = 0;
+  cudaMemset(ctx->dev_bad(), 0, sizeof(int));
+  cudaDeviceSynchronize();
+  cudaGetLastError();
+  return fail(ctx, KQ_ERR_INVALID_ARG,
+              "a paged-cache call met %s (code %d); nothing was read or written there and that sequence's output is "
+              "invalid",
+              code == 51   ? "a page outside the pool"
+              : code == 52 ? "a sequence length outside its block table"
+                           : "a row whose sequence or slot lies outside the block table",
+              code);
 }
 
-int finish_sync(kq_ctx* ctx, const char* what) {
-  cudaError_t e = stage_error_word(ctx);
+// Stream-ordered copy of the device error words into the pinned mirror.
+cudaError_t stage_error_words(kq_ctx* ctx) {
+  return cudaMemcpyAsync(ctx->host_err, ctx->dev_err, 2 * sizeof(int), cudaMemcpyDeviceToHost, ctx->stream);
+}
+
+int wait_for_stream(kq_ctx* ctx, const char* what) {
+  cudaError_t e = stage_error_words(ctx);
   if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->stream);
-  if (e != cudaSuccess) return cuda_fail(ctx, e, what);
-  return check_device_error(ctx);
+  return e == cudaSuccess ? KQ_OK : cuda_fail(ctx, e, what);
+}
+
+// End of a synchronous call: bad input of paged-cache calls before it is none of its
+// errors and stays for kq_ctx_synchronize.
+int finish_sync(kq_ctx* ctx, const char* what) {
+  const int rc = wait_for_stream(ctx, what);
+  return rc ? rc : check_wait_error(ctx);
 }
 
 // The CUDA-core f32 kernel of Q2_K / Q3_K / Q5_K (kq_kx.cu): internal
@@ -339,9 +358,9 @@ int kq_ctx_create(int device, kq_ctx** out) {
   ctx->device = device;
   cudaDeviceGetAttribute(&ctx->num_sms, cudaDevAttrMultiProcessorCount, device);
   e = cudaStreamCreateWithFlags(&ctx->own_stream, cudaStreamNonBlocking);
-  if (e == cudaSuccess) e = cudaMalloc(&ctx->dev_err, sizeof(int));
-  if (e == cudaSuccess) e = cudaMemset(ctx->dev_err, 0, sizeof(int));
-  if (e == cudaSuccess) e = cudaHostAlloc(&ctx->host_err, sizeof(int), cudaHostAllocDefault);
+  if (e == cudaSuccess) e = cudaMalloc(&ctx->dev_err, 2 * sizeof(int));
+  if (e == cudaSuccess) e = cudaMemset(ctx->dev_err, 0, 2 * sizeof(int));
+  if (e == cudaSuccess) e = cudaHostAlloc(&ctx->host_err, 2 * sizeof(int), cudaHostAllocDefault);
   if (e != cudaSuccess) {
     if (ctx->own_stream) cudaStreamDestroy(ctx->own_stream);
     if (ctx->dev_err) cudaFree(ctx->dev_err);
@@ -349,7 +368,7 @@ int kq_ctx_create(int device, kq_ctx** out) {
     cudaGetLastError();
     return KQ_ERR_CUDA;
   }
-  *ctx->host_err = 0;
+  ctx->host_err[0] = ctx->host_err[1] = 0;
   ctx->stream = ctx->own_stream;
   *out = ctx;
   return KQ_OK;
@@ -418,7 +437,13 @@ int kq_ctx_prefetch_next(kq_ctx* ctx, const kq_weight* next) {
 int kq_ctx_synchronize(kq_ctx* ctx) {
   if (check_ctx(ctx)) return KQ_ERR_INVALID_ARG;
   DeviceGuard g(ctx->device);
-  return finish_sync(ctx, "cudaStreamSynchronize");
+  if (const int rc = wait_for_stream(ctx, "cudaStreamSynchronize")) return rc;
+  // a wait that gave up is the graver one: its message goes first, the other is kept in it
+  const int bad = check_bad_input(ctx);
+  const std::string message = bad ? ctx->err : std::string();
+  const int rc = check_wait_error(ctx);
+  if (rc && bad) ctx->err += "; also " + message;
+  return rc ? rc : bad;
 }
 
 int kq_ctx_reserve(kq_ctx* ctx, const kq_weight* w, int64_t m) {
@@ -1372,7 +1397,7 @@ int kq_kv_append(kq_kv* kv, const float* qkv, int64_t ld, int64_t rows, int head
   a.q_ld = q_ld;
   a.slot_pos = slot_pos;
   a.track_ld = track_ld;
-  a.err = ctx->dev_err;
+  a.bad = ctx->dev_bad();
   DeviceGuard g(ctx->device);
   if (g.status != cudaSuccess) return cuda_fail(ctx, g.status, "cudaSetDevice");
   const cudaError_t e = kq::kv_append(a, ctx->stream);
@@ -1426,6 +1451,7 @@ static int kv_attention_impl(kq_kv* kv, const char* what, bool rope, const float
   a.scratch = scratch;
   a.num_sms = ctx->num_sms;
   a.err = ctx->dev_err;
+  a.bad = ctx->dev_bad();
   DeviceGuard g(ctx->device);
   if (g.status != cudaSuccess) return cuda_fail(ctx, g.status, "cudaSetDevice");
   int launches = 0;
@@ -1484,7 +1510,7 @@ int kq_kv_evict(kq_kv* kv, int64_t batch, const int32_t* table, int64_t table_ld
   a.keep = keep;
   a.scratch = scratch;
   a.num_sms = ctx->num_sms;
-  a.err = ctx->dev_err;
+  a.bad = ctx->dev_bad();
   DeviceGuard g(ctx->device);
   if (g.status != cudaSuccess) return cuda_fail(ctx, g.status, "cudaSetDevice");
   int launches = 0;

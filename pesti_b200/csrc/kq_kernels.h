@@ -384,7 +384,7 @@ struct KvAppendArgs {
   int64_t q_ld;
   int32_t* slot_pos;  // [batch][hkv][track_ld], or NULL
   int64_t track_ld;
-  int* err;
+  int* bad;  // the context's word for input out of bounds
 };
 cudaError_t kv_append(const KvAppendArgs& a, cudaStream_t s);
 struct KvAttnArgs {
@@ -405,7 +405,8 @@ struct KvAttnArgs {
   int64_t track_ld;
   void* scratch;
   int num_sms;
-  int* err;
+  int* err;  // the context's words for waits that gave up
+  int* bad;  // and for input out of bounds
 };
 // head_dim 64, 128 or 256, 1 to KV_MAX_GROUP query heads per kv head.
 constexpr int KV_MAX_GROUP = 16;
@@ -427,7 +428,7 @@ struct KvEvictArgs {
   int32_t keep;
   void* scratch;
   int num_sms;
-  int* err;
+  int* bad;  // the context's word for input out of bounds
 };
 size_t kv_evict_scratch_bytes(int64_t batch, int hkv, int64_t track_ld);
 cudaError_t kv_evict(const KvEvictArgs& a, int* launches, cudaStream_t s);

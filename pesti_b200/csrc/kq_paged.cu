@@ -70,7 +70,7 @@ __global__ void __launch_bounds__(AP_THREADS, 8) kv_append_kernel(const KvAppend
   const int64_t b = slot >= 0 && A.seqs ? A.seqs[r] : r;
   const bool bad = slot < -1 || (slot >= 0 && (b < 0 || b >= A.batch || slot >= A.table_ld * A.pool.page_size ||
                                                (A.slot_pos && slot >= A.track_ld)));
-  if (bad && tid == 0) kv_error(A.err, KV_ERR_ROW);
+  if (bad && tid == 0) kv_error(A.bad, KV_ERR_ROW);
   const bool live = slot >= 0 && !bad;
   int32_t pos = 0;
   int64_t row0 = -1;
@@ -84,7 +84,7 @@ __global__ void __launch_bounds__(AP_THREADS, 8) kv_append_kernel(const KvAppend
       reinterpret_cast<float*>(turn_s)[i] = (float)s;
     }
     row0 = kv_row(A.pool, page, slot, 0);
-    if (row0 < 0 && tid == 0) kv_error(A.err, KV_ERR_PAGE);
+    if (row0 < 0 && tid == 0) kv_error(A.bad, KV_ERR_PAGE);
   }
   __syncthreads();
   if (!live) return;
@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(EV_THREADS, 2) kv_evict_select_kernel(const Kv
   kv_pdl_enter();
   bool bad;
   const int len = (int)kv_len(A.lens[b], min(A.table_ld * A.pool.page_size, A.track_ld), &bad);
-  if (bad && tid == 0) kv_error(A.err, KV_ERR_LEN);
+  if (bad && tid == 0) kv_error(A.bad, KV_ERR_LEN);
   const int keep = A.keep, new_len = min(len, keep);
   const int share = (int)(((int64_t)len + CL - 1) / CL), s0 = min(len, part * share), n = min(len, s0 + share) - s0;
   EvictPlan* plan = static_cast<EvictPlan*>(A.scratch) + bh;
@@ -422,7 +422,7 @@ __global__ void __launch_bounds__(EV_MOVERS, 4) kv_evict_move_kernel(const KvEvi
     int64_t at = -1;
     if (mine < rows) {
       at = kv_row(A.pool, table[slot / A.pool.page_size], slot, hk);
-      if (at < 0) kv_error(A.err, KV_ERR_PAGE);
+      if (at < 0) kv_error(A.bad, KV_ERR_PAGE);
       if (from) {  // the mover's weight and position go with its row
         A.mass_out[bh * A.track_ld + hole] = A.mass[bh * A.track_ld + slot];
         A.pos_out[bh * A.track_ld + hole] = A.slot_pos[bh * A.track_ld + slot];

@@ -9,7 +9,8 @@
 
 namespace kq {
 
-// Device error codes of the paged cache and its callers (the context's error word).
+// Device error codes of the paged cache: input out of bounds (a word that no wait
+// polls: other calls on the context go on as they are), and a wait that gave up.
 enum : int { KV_ERR_PAGE = 51, KV_ERR_LEN = 52, KV_ERR_ROW = 53, KV_ERR_WAIT = 54 };
 
 // A sequence's slots in use; where lens[b] is outside [0, most], *bad is set and the
@@ -32,7 +33,7 @@ __device__ __forceinline__ void kv_pdl_enter() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
-__device__ __forceinline__ void kv_error(int* err, int code) { atomicCAS(err, 0, code); }
+__device__ __forceinline__ void kv_error(int* bad, int code) { atomicCAS(bad, 0, code); }
 
 // Turns (of a full circle) per position of pair i: theta^(-i / half) / (2 pi).
 __device__ __forceinline__ double rope_freq(int i, int half, double log2_theta) {

@@ -309,7 +309,7 @@ __global__ void __launch_bounds__(PaCfg<HD, NS>::THREADS, PaCfg<HD, NS>::CTAS)
         __syncwarp();
         if (i < valid) {
           // a page outside the pool is outside the descriptor: the box is filled with zeros
-          if (page_now < 0 || page_now >= A.pool.pages) kv_error(A.err, KV_ERR_PAGE);
+          if (page_now < 0 || page_now >= A.pool.pages) kv_error(A.bad, KV_ERR_PAGE);
           tma_load_5d(sm + s * C::STAGE + (is_v ? C::TILE_B : 0) + i * P.box * HD * 2, is_v ? &vmap : &kmap, row_now,
                       W.hk, page_now, full + s);
         }
@@ -343,7 +343,7 @@ __global__ void __launch_bounds__(PaCfg<HD, NS>::THREADS, PaCfg<HD, NS>::CTAS)
     bool bad;
     if (pa_len(A, b, &bad) == 0)
       for (int e = tid; e < A.hq * HD; e += C::CW * 32) A.out[b * A.out_ld + e] = 0.f;
-    if (bad && tid == 0) kv_error(A.err, KV_ERR_LEN);
+    if (bad && tid == 0) kv_error(A.bad, KV_ERR_LEN);
   }
 
   // lane's places in a 16-slot group, swizzled: rows of K (M rows, two k8 halves) and of V

@@ -1,0 +1,50 @@
+"""Calls of the paged cache as a server mixes them on one context: what one call
+leaves behind for the next, block tables cut out of wider ones, infinite keys,
+and what the calls do with the sequences that are in order beside one that is
+not.  Definitions and tolerances are those of test_gpu_paged."""
+import pytest
+import torch
+
+from pesti_b200 import decoder as dec
+from pesti_b200 import kq, synthetic
+from test_gpu_paged import DEV, Setup, status
+from test_gpu_serving import LLAMA_TINY
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- input out of bounds and the calls behind it ---------------------------------------------
+
+
+def test_bad_input_leaves_the_other_calls_on_the_context_alone(gpu_ctx):
+    """A row past its table, then a whole decode step in one kernel (its grid barriers and
+    exchange words are waited for) and a synchronous linear, before anything is synchronized:
+    both as without the row, which the context's own synchronize reports, once."""
+    model = dec.Decoder(LLAMA_TINY, gpu_ctx, 1, 20, max_new=4, seed=5, step_kernel=True)
+    assert model.step_kernel
+    s = Setup(gpu_ctx, [40], 2, 2, 64, 16, seed=71)
+    table = s.table[:, :3].contiguous()
+    qkv = torch.randn((1, 6 * 64), generator=s.g, device=DEV)
+    slots = torch.tensor([48], dtype=torch.int32, device=DEV)
+    raw = synthetic.gguf_weight(kq.KQ_GGUF_Q4_K, 512, 1024, seed=1)
+    w = kq.Weight(gpu_ctx, kq.KQ_GGUF_Q4_K, raw, 512, 1024)
+    x, y, y2 = torch.randn((1, 1024), generator=s.g, device=DEV), torch.zeros(512, device=DEV), torch.zeros(512, device=DEV)
+    model.tokens.fill_(7)
+    torch.cuda.synchronize()
+    model.step(20)
+    w.linear(x, 1, y, device_ptrs=True, sync=True)
+    gpu_ctx.synchronize()
+    want = model.logits.clone()
+    for _ in range(20):
+        model.logits.fill_(9.0)
+        torch.cuda.synchronize()
+        s.cache.append(qkv, table, slots, theta=1e4)
+        for _ in range(4):  # the same step again: it writes the same row of its cache
+            model.step(20)
+        w.linear(x, 1, y2, device_ptrs=True, sync=True)
+        torch.cuda.synchronize()
+        assert torch.equal(model.logits, want) and torch.equal(y2, y)
+        assert status(gpu_ctx.synchronize) == kq.KQ_ERR_INVALID_ARG
+        gpu_ctx.synchronize()
+    w.free()
+    model.close()
