@@ -192,7 +192,8 @@ int kq_kv_destroy(kq_kv *kv);
 /* Rows of q (heads) | k (kv_heads) | v (kv_heads), ld floats apart, into the
  * cache: row r goes to slot slots[r] of sequence seqs[r] (NULL: sequence r), k
  * turned to position pos[r] (NULL: the slot) as in kq_dec_rope_append, with
- * the angle reduced in 64 bits, k and v rounded to f16.  slots[r] = -1 skips
+ * the angle reduced in 64 bits and k exact to the nearest f32 (the bits that
+ * kq_kv_rope_attention stores), k and v rounded to f16.  slots[r] = -1 skips
  * the row.  q_out (NULL: not needed; it may be qkv itself with q_ld = ld, else
  * it must not overlap it) receives the turned query heads.  slot_pos [batch][kv_heads][track_ld]
  * (NULL: not kept) receives the position of each written slot.  The slots of

@@ -21,7 +21,7 @@ namespace cg = cooperative_groups;
 // by the row's bytes: f32 in, f32 q and f16 k, v out.  Many small CTAs hide the chain
 // slot - page - row better than several steps' loads in flight: 4099 rows of 32 / 8
 // heads of 128 took 33.2 us with one step and eight CTAs per SM, 38.9 with four steps
-// and four (34.5 us, 5360 GB/s, since sines are 64-bit as well).
+// and four (a call takes 36.6 us, 5040 GB/s, since keys are exact; 35.8 with f32 sums).
 constexpr int AP_THREADS = 256, AP_MAX_HALF = 128;
 
 // Four floats at p, in one access where `vec` (p is then 16-byte aligned).
@@ -38,21 +38,43 @@ __device__ __forceinline__ void store4(float* p, float4 v, bool vec) {
     p[3] = v.w;
   }
 }
-__device__ __forceinline__ uint2 halves(float4 v) {
-  const __half2 a = __floats2half2_rn(v.x, v.y), b = __floats2half2_rn(v.z, v.w);
-  return make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+__device__ __forceinline__ uint32_t pair_bits(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint2 halves(float4 v) { return make_uint2(pair_bits(v.x, v.y), pair_bits(v.z, v.w)); }
+
+// Two pairs of a key turned and rounded to f16 as turn_key's are: in plain f32, and
+// where its error could round another way (one pair in 100) by exact_dot2.  The error:
+// c, s, the product rounded by itself and the sum each add 2^-24 of what they round,
+// together at most 3 x 2^-24 of the two products.  lo: what f32 leaves of the cosines,
+// and `half` behind that of the sines.  (4099 rows: a call 36.6 us; 37.6 by exact_dot2 alone.)
+__device__ __forceinline__ void turn_keys(float2 x, float2 y, float2 c, float2 s, const float* lo, int half,
+                                          uint32_t& a, uint32_t& b) {
+  constexpr float E = 0x1.8p-23f;
+  // x c + y s of both pairs, as two f16
+  auto dots = [&](float2 y, float2 c, const float* c_lo, float2 s, const float* s_lo) {
+    const float p0 = x.x * c.x, p1 = x.y * c.y;
+    const float a0 = fmaf(y.x, s.x, p0), a1 = fmaf(y.y, s.y, p1);
+    const float e0 = E * fmaf(fabsf(y.x), fabsf(s.x), fabsf(p0)), e1 = E * fmaf(fabsf(y.y), fabsf(s.y), fabsf(p1));
+    const uint32_t least = pair_bits(a0 - e0, a1 - e1);
+    if (least == pair_bits(a0 + e0, a1 + e1)) return least;
+    return pair_bits(exact_dot2(x.x, c.x, c_lo[0], y.x, s.x, s_lo[0]), exact_dot2(x.y, c.y, c_lo[1], y.y, s.y, s_lo[1]));
+  };
+  a = dots(make_float2(-y.x, -y.y), c, lo, s, lo + half);
+  b = dots(y, s, lo + half, c, lo);
 }
 
 template <int TPR>
 __global__ void __launch_bounds__(AP_THREADS, 8) kv_append_kernel(const KvAppendArgs A, bool vec_in, bool vec_out) {
-  extern __shared__ float4 turns[];  // per row of the CTA: hd / 2 cosines, then as many sines
+  extern __shared__ float4 turns[];  // per row of the CTA: hd / 2 cosines, as many sines, and what f32 leaves of both
   __shared__ double freq[AP_MAX_HALF];
   const int hd = A.pool.hd, half = hd / 2, hkv = A.pool.hkv, tid = threadIdx.x % TPR;
   if (threadIdx.x < half) freq[threadIdx.x] = rope_freq(threadIdx.x, half, A.log2_theta);
   __syncthreads();
   kv_pdl_enter();
   const int64_t r = (int64_t)blockIdx.x * (AP_THREADS / TPR) + threadIdx.x / TPR;
-  float4* turn_c = turns + (threadIdx.x / TPR) * (half / 2);
+  float4* turn_c = turns + (threadIdx.x / TPR) * half;
   float4* turn_s = turn_c + half / 4;
   // q and k heads in quads of pairs (q only where it is wanted); the first loads come
   // before the row's place is known
@@ -80,8 +102,11 @@ __global__ void __launch_bounds__(AP_THREADS, 8) kv_append_kernel(const KvAppend
     for (int i = tid; i < half; i += TPR) {
       double c, s;
       rope_turn(pos, freq[i], c, s);
-      reinterpret_cast<float*>(turn_c)[i] = (float)c;
-      reinterpret_cast<float*>(turn_s)[i] = (float)s;
+      float* to = reinterpret_cast<float*>(turn_c) + i;
+      to[0] = (float)c;
+      to[half] = (float)s;
+      to[2 * half] = (float)(c - (double)to[0]);
+      to[3 * half] = (float)(s - (double)to[half]);
     }
     row0 = kv_row(A.pool, page, slot, 0);
     if (row0 < 0 && tid == 0) kv_error(A.bad, KV_ERR_PAGE);
@@ -96,18 +121,24 @@ __global__ void __launch_bounds__(AP_THREADS, 8) kv_append_kernel(const KvAppend
     if (e != first + tid) load(e);
     const int head = e / quads, i = 4 * (e % quads);
     const float4 c = turn_c[i / 4], s = turn_s[i / 4];
-    const float4 a = make_float4(x.x * c.x - y.x * s.x, x.y * c.y - y.y * s.y, x.z * c.z - y.z * s.z,
-                                 x.w * c.w - y.w * s.w);
-    const float4 d = make_float4(x.x * s.x + y.x * c.x, x.y * s.y + y.y * c.y, x.z * s.z + y.z * c.z,
-                                 x.w * s.w + y.w * c.w);
     if (head < A.hq) {
+      const float4 a = make_float4(x.x * c.x - y.x * s.x, x.y * c.y - y.y * s.y, x.z * c.z - y.z * s.z,
+                                   x.w * c.w - y.w * s.w);
+      const float4 d = make_float4(x.x * s.x + y.x * c.x, x.y * s.y + y.y * c.y, x.z * s.z + y.z * c.z,
+                                   x.w * s.w + y.w * c.w);
       float* o = q_out + (int64_t)head * hd + i;
       store4(o, a, vec_out);
       store4(o + half, d, vec_out);
     } else if (row0 >= 0) {
+      const float* lo = reinterpret_cast<const float*>(turn_c) + 2 * half + i;
+      uint2 a, d;
+      turn_keys(make_float2(x.x, x.y), make_float2(y.x, y.y), make_float2(c.x, c.y), make_float2(s.x, s.y), lo, half,
+                a.x, d.x);
+      turn_keys(make_float2(x.z, x.w), make_float2(y.z, y.w), make_float2(c.z, c.w), make_float2(s.z, s.w), lo + 2,
+                half, a.y, d.y);
       __half* o = kc + (head - A.hq) * head_ld + i;
-      *reinterpret_cast<uint2*>(o) = halves(a);
-      *reinterpret_cast<uint2*>(o + half) = halves(d);
+      *reinterpret_cast<uint2*>(o) = a;
+      *reinterpret_cast<uint2*>(o + half) = d;
     }
   }
   if (row0 < 0) return;
@@ -460,7 +491,7 @@ cudaError_t kv_append(const KvAppendArgs& a, cudaStream_t s) {
   auto launch = [&](auto kernel, int tpr) {
     const int rows = AP_THREADS / tpr;
     return launch_pdl(kernel, dim3((unsigned)((a.rows + rows - 1) / rows)), dim3(AP_THREADS),
-                      (size_t)rows * hd * sizeof(float), s, a, vec_in, vec_out);
+                      (size_t)rows * 2 * hd * sizeof(float), s, a, vec_in, vec_out);
   };
   if (steps <= 16 * 4) return launch(kv_append_kernel<16>, 16);
   if (steps <= 32 * 4) return launch(kv_append_kernel<32>, 32);

@@ -54,6 +54,23 @@ __device__ __forceinline__ void rope_turn(int32_t pos, double freq, double& c, d
   c = quarter == 1 || quarter == 2 ? -a : a;
   s = quarter & 2 ? -b : b;
 }
+// x c + y s to the nearest f32, c and s given as two f32 parts: the products' and the
+// sum's roundings are worked out (a product's by fma, a sum's by Knuth's two-sum) and
+// added last, 2^-46 of |x c| + |y s| is left.  Plain f32 sums would round another way
+// to f16 at 2e-4 of the elements; FP64 takes more of the append kernel's 32 registers.
+__device__ __forceinline__ float exact_dot2(float x, float c, float c_lo, float y, float s, float s_lo) {
+  const float p = __fmul_rn(x, c), q = __fmul_rn(y, s), sum = __fadd_rn(p, q);
+  const float z = __fsub_rn(sum, p), lost = __fadd_rn(__fsub_rn(p, __fsub_rn(sum, z)), __fsub_rn(q, z));
+  const float pe = __fmaf_rn(x, c_lo, __fmaf_rn(x, c, -p)), qe = __fmaf_rn(y, s_lo, __fmaf_rn(y, s, -q));
+  const float r = __fadd_rn(sum, __fadd_rn(lost, __fadd_rn(pe, qe)));
+  return isfinite(sum) ? r : sum;
+}
+// A key's pair (x, y) turned.
+__device__ __forceinline__ void turn_key(float x, float y, float c, float c_lo, float s, float s_lo, float& a,
+                                         float& b) {
+  a = exact_dot2(x, c, c_lo, -y, s, s_lo);
+  b = exact_dot2(x, s, s_lo, y, c, c_lo);
+}
 #endif
 
 }  // namespace kq

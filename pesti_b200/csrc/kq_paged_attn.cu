@@ -455,15 +455,11 @@ __global__ void __launch_bounds__(PaCfg<HD, NS>::THREADS, PaCfg<HD, NS>::CTAS)
         for (int k = 0; k < IN; ++k) {
           const int i = qi + 64 * k;
           __half2 a, b;
-          if (w == 0) {  // in 64 bits to the nearest f32 (sums in f32 would round another way to f16 at 2e-4 of them)
+          if (w == 0) {
             float ab[2][2];
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const double co = (double)cs[k][e] + cs_lo[k][e], si = (double)sn[k][e] + sn_lo[k][e];
-              const double x = nr[k][e], y = nr[k][e + 2];
-              ab[0][e] = (float)(x * co - y * si);
-              ab[1][e] = (float)(x * si + y * co);
-            }
+            for (int e = 0; e < 2; ++e)
+              turn_key(nr[k][e], nr[k][e + 2], cs[k][e], cs_lo[k][e], sn[k][e], sn_lo[k][e], ab[0][e], ab[1][e]);
             a = __floats2half2_rn(ab[0][0], ab[0][1]);
             b = __floats2half2_rn(ab[1][0], ab[1][1]);
           } else {

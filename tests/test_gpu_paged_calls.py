@@ -6,8 +6,8 @@ import pytest
 import torch
 
 from pesti_b200 import decoder as dec
-from pesti_b200 import kq, synthetic
-from test_gpu_paged import DEV, Setup, status
+from pesti_b200 import kq, paged, synthetic
+from test_gpu_paged import DEV, Setup, status, turn
 from test_gpu_serving import LLAMA_TINY
 
 pytestmark = pytest.mark.gpu
@@ -48,3 +48,42 @@ def test_bad_input_leaves_the_other_calls_on_the_context_alone(gpu_ctx):
         gpu_ctx.synchronize()
     w.free()
     model.close()
+
+
+# ---- appended keys ------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("hd,hkv", [(64, 1), (64, 4), (128, 8), (256, 2)])
+def test_append_stores_the_exact_key_rounded(gpu_ctx, hd, hkv):
+    """As for a step's key: turned in 64 bits, to the nearest f32, to the nearest f16.  The
+    first rounding moves the second at about 1e-7 of the elements; sums in f32 would move 2e-4 of
+    them, some fifty of these 262,144."""
+    n, hq, theta = 262144 // (hd * hkv), hkv, 1e6
+    s = Setup(gpu_ctx, [n], hq, hkv, hd, 16, seed=hd)
+    qkv = torch.randn((n, (hq + 2 * hkv) * hd), generator=s.g, device=DEV)
+    pos = torch.randint(0, 120000, (n,), generator=s.g, device=DEV).int()
+    slots, seqs = torch.arange(n, dtype=torch.int32, device=DEV), torch.zeros(n, dtype=torch.int32, device=DEV)
+    torch.cuda.synchronize()
+    s.cache.append(qkv, s.table, slots, theta=theta, seqs=seqs, pos=pos)
+    gpu_ctx.synchronize()
+    want = turn(qkv.view(n, hq + 2 * hkv, hd)[:, hq:hq + hkv], pos, theta).half()
+    at = s.table[0, slots.long() // 16].long()
+    assert int((s.k[at, :, slots.long() % 16] != want).sum()) <= 2
+
+
+@pytest.mark.parametrize("hd,hq,hkv", [(64, 14, 2), (128, 32, 8), (256, 9, 1)])
+def test_append_and_a_step_store_the_same_keys(gpu_ctx, hd, hq, hkv):
+    """A token that is appended again later finds the bits that its own step wrote."""
+    B, theta = 400, 5e5
+    s = Setup(gpu_ctx, [3] * B, hq, hkv, hd, 16, seed=hd + 1)
+    qkv = 3.0 * torch.randn((B, (hq + 2 * hkv) * hd), generator=s.g, device=DEV)
+    pos = torch.randint(0, 1 << 20, (B,), generator=s.g, device=DEV).int()
+    out = torch.zeros((B, hq * hd), device=DEV)
+    again = paged.PagedCache(gpu_ctx, s.k.clone(), s.v.clone())
+    scratch = s.cache.scratch(B, hq)
+    torch.cuda.synchronize()
+    s.cache.rope_attention(qkv, s.table, s.lens, out, scratch, theta=theta, pos=pos)
+    again.append(qkv, s.table, s.lens - 1, theta=theta, pos=pos)
+    gpu_ctx.synchronize()
+    at = s.table[:, 0].long()
+    assert torch.equal(s.k[at, :, 2], again.k[at, :, 2]) and torch.equal(s.v[at, :, 2], again.v[at, :, 2])
