@@ -202,6 +202,15 @@ int kq_kv_destroy(kq_kv *kv);
 int kq_kv_append(kq_kv *kv, const float *qkv, int64_t ld, int64_t rows, int heads, const int32_t *seqs,
                  const int32_t *slots, const int32_t *pos, const int32_t *table, int64_t table_ld, int64_t batch,
                  float theta, float *q_out, int64_t q_ld, int32_t *slot_pos, int64_t track_ld);
+/* The same for caches whose attention weights are accumulated: mass [batch]
+ * [kv_heads][track_ld] (NULL: not kept) starts at 0 at each written slot.  An
+ * eviction leaves the old weights of the slots that it frees in the array, and
+ * kq_kv_attention adds to what is there, so slots that are appended to without
+ * this keep the weight of whatever lay there before. */
+int kq_kv_append_tracked(kq_kv *kv, const float *qkv, int64_t ld, int64_t rows, int heads, const int32_t *seqs,
+                         const int32_t *slots, const int32_t *pos, const int32_t *table, int64_t table_ld,
+                         int64_t batch, float theta, float *q_out, int64_t q_ld, float *mass, int32_t *slot_pos,
+                         int64_t track_ld);
 /* Scratch bytes of the two calls below (track_len: track_ld where mass is
  * given, else 0); 0 for sizes that they refuse.  256-byte aligned, zero-filled
  * before its first use (it holds arrival counters that every call leaves at

@@ -1368,6 +1368,14 @@ static bool bad_theta(float theta) { return !(theta > 0.f) || std::isinf(theta);
 int kq_kv_append(kq_kv* kv, const float* qkv, int64_t ld, int64_t rows, int heads, const int32_t* seqs,
                  const int32_t* slots, const int32_t* pos, const int32_t* table, int64_t table_ld, int64_t batch,
                  float theta, float* q_out, int64_t q_ld, int32_t* slot_pos, int64_t track_ld) {
+  return kq_kv_append_tracked(kv, qkv, ld, rows, heads, seqs, slots, pos, table, table_ld, batch, theta, q_out, q_ld,
+                              nullptr, slot_pos, track_ld);
+}
+
+int kq_kv_append_tracked(kq_kv* kv, const float* qkv, int64_t ld, int64_t rows, int heads, const int32_t* seqs,
+                         const int32_t* slots, const int32_t* pos, const int32_t* table, int64_t table_ld,
+                         int64_t batch, float theta, float* q_out, int64_t q_ld, float* mass, int32_t* slot_pos,
+                         int64_t track_ld) {
   if (!kv) return KQ_ERR_INVALID_ARG;
   kq_ctx* ctx = kv->ctx;
   const char* what = "kq_kv_append";
@@ -1376,7 +1384,7 @@ int kq_kv_append(kq_kv* kv, const float* qkv, int64_t ld, int64_t rows, int head
   if (int rc = kv_heads_check(kv, what, heads, batch)) return rc;
   const int64_t hd = kv->pool.hd;
   if (rows < 0 || rows > INT32_MAX || ld < (heads + 2 * (int64_t)kv->pool.hkv) * hd || (q_out && q_ld < heads * hd) ||
-      (q_out == qkv && q_ld != ld && rows > 1) || (slot_pos && track_ld < 1) || (!seqs && rows > batch) || bad_theta(theta))
+      (q_out == qkv && q_ld != ld && rows > 1) || ((mass || slot_pos) && track_ld < 1) || (!seqs && rows > batch) || bad_theta(theta))
     return fail(ctx, KQ_ERR_INVALID_ARG, "%s: %lld rows of %lld, q rows of %lld, theta %g", what, (long long)rows,
                 (long long)ld, (long long)q_ld, (double)theta);
   if (rows == 0) return KQ_OK;
@@ -1395,6 +1403,7 @@ int kq_kv_append(kq_kv* kv, const float* qkv, int64_t ld, int64_t rows, int head
   a.log2_theta = std::log2((double)theta);
   a.q_out = q_out;
   a.q_ld = q_ld;
+  a.mass = mass;
   a.slot_pos = slot_pos;
   a.track_ld = track_ld;
   a.bad = ctx->dev_bad();

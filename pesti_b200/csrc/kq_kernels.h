@@ -382,7 +382,8 @@ struct KvAppendArgs {
   double log2_theta;
   float* q_out;  // NULL: q is not needed
   int64_t q_ld;
-  int32_t* slot_pos;  // [batch][hkv][track_ld], or NULL
+  float* mass;        // [batch][hkv][track_ld], each or NULL: a written slot's weight
+  int32_t* slot_pos;  // starts at 0, its position is noted
   int64_t track_ld;
   int* bad;  // the context's word for input out of bounds
 };

@@ -91,7 +91,7 @@ __global__ void __launch_bounds__(AP_THREADS, 8) kv_append_kernel(const KvAppend
   const int32_t slot = r < A.rows ? A.slots[r] : -1;
   const int64_t b = slot >= 0 && A.seqs ? A.seqs[r] : r;
   const bool bad = slot < -1 || (slot >= 0 && (b < 0 || b >= A.batch || slot >= A.table_ld * A.pool.page_size ||
-                                               (A.slot_pos && slot >= A.track_ld)));
+                                               ((A.slot_pos || A.mass) && slot >= A.track_ld)));
   if (bad && tid == 0) kv_error(A.bad, KV_ERR_ROW);
   const bool live = slot >= 0 && !bad;
   int32_t pos = 0;
@@ -146,8 +146,11 @@ __global__ void __launch_bounds__(AP_THREADS, 8) kv_append_kernel(const KvAppend
     const int h = e / (hd / 4), i = 4 * (e - h * (hd / 4));
     *reinterpret_cast<uint2*>(vc + h * head_ld + i) = halves(load4(row + (int64_t)(A.hq + hkv + h) * hd + i, vec_in));
   }
-  if (A.slot_pos)
-    for (int h = tid; h < hkv; h += TPR) A.slot_pos[(b * hkv + h) * A.track_ld + slot] = pos;
+  for (int h = tid; h < hkv; h += TPR) {
+    const int64_t at = (b * hkv + h) * A.track_ld + slot;
+    if (A.mass) A.mass[at] = 0.f;
+    if (A.slot_pos) A.slot_pos[at] = pos;
+  }
 }
 
 // ---- eviction ---------------------------------------------------------------------

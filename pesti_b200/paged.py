@@ -22,6 +22,7 @@ def _bind(lib: ctypes.CDLL) -> ctypes.CDLL:
         "kq_kv_create": ([P, P, P, I64, I64, I, I, I, ctypes.POINTER(P)], I),
         "kq_kv_destroy": ([P], I),
         "kq_kv_append": ([P, P, I64, I64, I, P, P, P, P, I64, I64, F, P, I64, P, I64], I),
+        "kq_kv_append_tracked": ([P, P, I64, I64, I, P, P, P, P, I64, I64, F, P, I64, P, P, I64], I),
         "kq_kv_attention_scratch": ([P, I64, I, I64], Z),
         "kq_kv_attention": ([P, P, I64, P, I64, I64, I, P, I64, P, P, I64, P, Z], I),
         "kq_kv_rope_attention": ([P, P, I64, P, I64, I64, I, P, I64, P, P, F, P, P, I64, P, Z], I),
@@ -62,7 +63,7 @@ class PagedCache:
         ctx.check(self.lib.kq_kv_create(ctx.handle, k.data_ptr(), v.data_ptr(), self.pages, page_ld,
                                         self.page_size, self.kv_heads, self.head_dim, ctypes.byref(h)), "kq_kv_create")
         self.handle = h
-        self._append, self._attention = self.lib.kq_kv_append, self.lib.kq_kv_attention
+        self._append, self._attention = self.lib.kq_kv_append_tracked, self.lib.kq_kv_attention
         self._rope_attention = self.lib.kq_kv_rope_attention
 
     # ---- argument checks (lean: they run before every call) ------------------------------
@@ -121,10 +122,13 @@ class PagedCache:
             raise _invalid(f"eviction from {batch} sequences of {track_ld} tracked slots")
         return torch.empty(n, dtype=torch.uint8, device=self.device)
 
-    def append(self, qkv, table, slots, *, theta: float, seqs=None, pos=None, q_out=None, slot_pos=None) -> None:
+    def append(self, qkv, table, slots, *, theta: float, seqs=None, pos=None, q_out=None, mass=None,
+               slot_pos=None) -> None:
         """Row r of qkv [rows][(heads + 2 kv_heads) head_dim] (q | k | v) into
         slot slots[r] (-1: none) of sequence seqs[r] (default r), turned to
-        position pos[r] (default: the slot); the turned q into q_out."""
+        position pos[r] (default: the slot); the turned q into q_out.  The
+        slots' mass starts at 0 (without it a slot used before keeps the weight
+        of what lay there), and their positions go to slot_pos."""
         f32, i32 = self._types
         ld, table_ld = self._rows(qkv, "qkv", f32), self._rows(table, "table", i32)
         rows, cols = qkv.shape
@@ -137,11 +141,14 @@ class PagedCache:
             q_ptr, q_ld = q_out.data_ptr(), self._rows(q_out, "q_out", f32, rows)
             if q_out.shape[1] < heads * hd:
                 raise _invalid(f"q_out: rows of {q_out.shape[1]} for {heads} heads of {hd}")
-        sp, track = (None, 0) if slot_pos is None else self._track(slot_pos, "slot_pos", i32, batch)
+        m, track = (None, 0) if mass is None else self._track(mass, "mass", f32, batch)
+        sp = None
+        if slot_pos is not None:
+            sp, track = self._track(slot_pos, "slot_pos", i32, batch, track)
         rc = self._append(self.handle, qkv.data_ptr(), ld, rows, heads,
                           None if seqs is None else self._vector(seqs, "seqs", rows),
                           self._vector(slots, "slots", rows), None if pos is None else self._vector(pos, "pos", rows),
-                          table.data_ptr(), table_ld, batch, theta, q_ptr, q_ld, sp, track)
+                          table.data_ptr(), table_ld, batch, theta, q_ptr, q_ld, m, sp, track)
         if rc:
             self.ctx.check(rc, "kq_kv_append")
 

@@ -2,12 +2,13 @@
 leaves behind for the next, block tables cut out of wider ones, infinite keys,
 and what the calls do with the sequences that are in order beside one that is
 not.  Definitions and tolerances are those of test_gpu_paged."""
+import numpy as np
 import pytest
 import torch
 
 from pesti_b200 import decoder as dec
 from pesti_b200 import kq, paged, synthetic
-from test_gpu_paged import DEV, Setup, status, turn
+from test_gpu_paged import DEV, TOL_OUT, Setup, keep_of, status, turn
 from test_gpu_serving import LLAMA_TINY
 
 pytestmark = pytest.mark.gpu
@@ -87,3 +88,80 @@ def test_append_and_a_step_store_the_same_keys(gpu_ctx, hd, hq, hkv):
     gpu_ctx.synchronize()
     at = s.table[:, 0].long()
     assert torch.equal(s.k[at, :, 2], again.k[at, :, 2]) and torch.equal(s.v[at, :, 2], again.v[at, :, 2])
+
+
+# ---- weights of slots that are used again ----------------------------------------------------
+
+
+def test_appended_slots_start_without_weight(gpu_ctx):
+    """Evict, append a chunk into the freed slots, attend, evict: the new slots are ranked by the
+    weights they gathered themselves, not by those of the tokens that lay there."""
+    hd, hq, hkv, page, lens, keep, more = 64, 4, 2, 16, [60, 45], 20, 12
+    s = Setup(gpu_ctx, lens, hq, hkv, hd, page, seed=21)
+    B, ld = 2, 64
+    spos = torch.arange(ld, dtype=torch.int32, device=DEV).expand(B, hkv, ld).contiguous()
+    mass = torch.rand((B, hkv, ld), generator=s.g, device=DEV)
+    mass[:, :, keep:] += 100.0  # cut off, these weights stay behind in the array
+    mass[:, :, :keep] += 200.0
+    chunk = torch.randn((B * more, (hq + 2 * hkv) * hd), generator=s.g, device=DEV)
+    q = torch.randn((B, hq * hd), generator=s.g, device=DEV)
+    seqs = torch.arange(B, dtype=torch.int32, device=DEV).repeat_interleave(more)
+    slots = (keep + torch.arange(more, dtype=torch.int32, device=DEV)).repeat(B)
+    slots[more - 1] = -1  # a row that is left out
+    grown = torch.tensor([keep + more - 1, keep + more], dtype=torch.int32, device=DEV)
+    out, scratch, es = torch.empty_like(q), s.cache.scratch(B, hq, ld), s.cache.evict_scratch(B, ld)
+    torch.cuda.synchronize()
+    s.cache.evict(s.table, s.lens, s.lens, mass, spos, mass, spos, keep, es)
+    gpu_ctx.synchronize()
+    old = mass.clone()
+    s.cache.append(chunk, s.table, slots, theta=1e4, seqs=seqs, pos=slots + 100, mass=mass, slot_pos=spos)
+    gpu_ctx.synchronize()
+    want = old.clone()
+    for b, n in enumerate(grown.tolist()):
+        want[b, :, keep:n] = 0.0
+    assert torch.equal(mass, want)
+    assert (spos[1, :, keep:keep + more] == slots[more:] + 100).all() and (spos[0, :, keep + more - 1] < 100).all()
+    s.lens_h, s.lens = grown.tolist(), grown
+    torch.cuda.synchronize()
+    s.cache.attention(q, s.table, s.lens, out, scratch, mass=mass)
+    gpu_ctx.synchronize()
+    _, ref = s.reference(q.view(B, hq, hd))
+    for (b, h), m in ref.items():
+        # the weight's own bound, and half a step of f32 of a sum near 200
+        assert float((mass[b, h, :len(m)] - want[b, h, :len(m)] - m).abs().max()) <= TOL_OUT * 2 + 2 ** -16
+    m0 = mass.cpu().numpy()
+    s.cache.evict(s.table, s.lens, s.lens, mass, spos, mass, spos, keep + 5, es)
+    gpu_ctx.synchronize()
+    for b, n in enumerate([keep + more - 1, keep + more]):
+        for h in range(hkv):
+            src = keep_of(m0[b, h, :n], np.arange(n), 1 << 40, keep + 5)
+            assert np.array_equal(src[:keep], np.arange(keep))  # the old slots, at 200 and more
+            assert np.array_equal(mass[b, h, :keep + 5].cpu().numpy(), m0[b, h, src])
+
+
+def test_append_checks_the_tracked_slots(gpu_ctx):
+    """mass alone, slot_pos alone, and slots past what is tracked."""
+    hd, hkv = 64, 2
+    s = Setup(gpu_ctx, [40, 30], 2, hkv, hd, 16, seed=22)
+    qkv = torch.randn((2, 6 * hd), generator=s.g, device=DEV)
+    slots = torch.tensor([39, 7], dtype=torch.int32, device=DEV)
+    mass = torch.ones((2, hkv, 40), device=DEV)
+    torch.cuda.synchronize()
+    s.cache.append(qkv, s.table, slots, theta=1e4, mass=mass)
+    gpu_ctx.synchronize()
+    want = torch.ones_like(mass)
+    want[0, :, 39] = want[1, :, 7] = 0.0
+    assert torch.equal(mass, want)
+    short = torch.ones((2, hkv, 39), device=DEV)
+    k0 = s.k.clone()
+    torch.cuda.synchronize()
+    s.cache.append(3 * qkv, s.table, slots, theta=1e4, mass=short)
+    assert status(gpu_ctx.synchronize) == kq.KQ_ERR_INVALID_ARG  # slot 39 of 39: that row is left out
+    assert (short[0] == 1).all() and (short[1, :, 7] == 0).all() and int((short == 0).sum()) == hkv
+    at = int(s.table[0, 2])
+    assert torch.equal(s.k[at].nan_to_num(7), k0[at].nan_to_num(7))
+    bad = kq.KQ_ERR_INVALID_ARG
+    spos = torch.zeros((2, hkv, 41), dtype=torch.int32, device=DEV)
+    assert status(s.cache.append, qkv, s.table, slots, theta=1e4, mass=mass, slot_pos=spos) == bad
+    assert status(s.cache.append, qkv, s.table, slots, theta=1e4, mass=mass.double()) == bad
+    assert status(s.cache.append, qkv, s.table, slots, theta=1e4, mass=mass[:1]) == bad
