@@ -189,6 +189,11 @@ typedef struct kq_kv kq_kv;
 int kq_kv_create(kq_ctx *ctx, void *k_pool, void *v_pool, int64_t pages, int64_t page_ld, int page_size, int kv_heads,
                  int head_dim, kq_kv **out);
 int kq_kv_destroy(kq_kv *kv);
+/* Block tables of the calls that follow have `cols` columns, which is what
+ * bounds lengths and slots, though their rows lie table_ld entries apart (a part
+ * of a wider table).  0, as created: table_ld columns.  A captured call keeps
+ * the width it was captured with. */
+int kq_kv_set_table_cols(kq_kv *kv, int64_t cols);
 /* Rows of q (heads) | k (kv_heads) | v (kv_heads), ld floats apart, into the
  * cache: row r goes to slot slots[r] of sequence seqs[r] (NULL: sequence r), k
  * turned to position pos[r] (NULL: the slot) as in kq_dec_rope_append, with

@@ -92,6 +92,7 @@ struct kq_kv {
   kq_ctx* ctx = nullptr;
   kq::KvPool pool;
   kq::KvMaps maps;
+  int64_t table_cols = 0;  // pages that a sequence has at most, 0: as many as a table's rows are apart
 };
 
 // A decode-step program (kq_step_*): its stages on the host, and once built,
@@ -1344,6 +1345,14 @@ int kq_kv_destroy(kq_kv* kv) {
   return KQ_OK;
 }
 
+int kq_kv_set_table_cols(kq_kv* kv, int64_t cols) {
+  if (!kv) return KQ_ERR_INVALID_ARG;
+  if (cols < 0 || cols > INT32_MAX)
+    return fail(kv->ctx, KQ_ERR_INVALID_ARG, "kq_kv_set_table_cols: %lld pages per sequence", (long long)cols);
+  kv->table_cols = cols;
+  return KQ_OK;
+}
+
 // The arguments every paged-cache call shares.
 static int kv_check(kq_kv* kv, const char* what, const int32_t* table, int64_t table_ld, int64_t batch) {
   kq_ctx* ctx = kv->ctx;
@@ -1399,6 +1408,7 @@ int kq_kv_append_tracked(kq_kv* kv, const float* qkv, int64_t ld, int64_t rows, 
   a.pos = pos;
   a.table = table;
   a.table_ld = table_ld;
+  a.table_cols = kv->table_cols ? kv->table_cols : table_ld;
   a.batch = batch;
   a.log2_theta = std::log2((double)theta);
   a.q_out = q_out;
@@ -1451,6 +1461,7 @@ static int kv_attention_impl(kq_kv* kv, const char* what, bool rope, const float
   a.hq = heads;
   a.table = table;
   a.table_ld = table_ld;
+  a.table_cols = kv->table_cols ? kv->table_cols : table_ld;
   a.lens = lens;
   a.pos = pos;
   a.log2_theta = rope ? std::log2((double)theta) : 0.0;
@@ -1508,6 +1519,7 @@ int kq_kv_evict(kq_kv* kv, int64_t batch, const int32_t* table, int64_t table_ld
   a.batch = batch;
   a.table = table;
   a.table_ld = table_ld;
+  a.table_cols = kv->table_cols ? kv->table_cols : table_ld;
   a.lens = lens;
   a.lens_out = lens_out;
   a.mass = mass;

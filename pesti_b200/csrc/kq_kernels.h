@@ -352,7 +352,8 @@ cudaError_t dec_embed(const float* table, const int* tokens, float* out, int64_t
 
 // ---- paged key-value cache: kq_paged.cu ----
 // Pools of `pages` pages, page_ld elements apart, each [kv_heads][page_size][hd]
-// f16.  Slot j of sequence b lies in page table[b * table_ld + j / page_size].
+// f16.  Slot j of sequence b lies in page table[b * table_ld + j / page_size]; a
+// sequence has table_cols pages at most.
 struct KvPool {
   void* k = nullptr;
   void* v = nullptr;
@@ -378,7 +379,7 @@ struct KvAppendArgs {
   const int32_t* slots;  // [rows] its slot, -1: the row is skipped
   const int32_t* pos;    // [rows] its rotary position (NULL: the slot)
   const int32_t* table;
-  int64_t table_ld, batch;
+  int64_t table_ld, table_cols, batch;
   double log2_theta;
   float* q_out;  // NULL: q is not needed
   int64_t q_ld;
@@ -397,7 +398,7 @@ struct KvAttnArgs {
   int64_t out_ld, batch;
   int hq;
   const int32_t* table;
-  int64_t table_ld;
+  int64_t table_ld, table_cols;
   const int32_t* lens;  // [batch] slots in use, the new one included; 0: an idle row
   const int32_t* pos;   // rope: [batch] the new token's position (NULL: lens - 1)
   double log2_theta;
@@ -417,7 +418,7 @@ struct KvEvictArgs {
   KvPool pool;
   int64_t batch;
   const int32_t* table;
-  int64_t table_ld;
+  int64_t table_ld, table_cols;
   const int32_t* lens;
   int32_t* lens_out;
   const float* mass;

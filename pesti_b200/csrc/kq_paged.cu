@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(AP_THREADS, 8) kv_append_kernel(const KvAppend
   load(first + tid);
   const int32_t slot = r < A.rows ? A.slots[r] : -1;
   const int64_t b = slot >= 0 && A.seqs ? A.seqs[r] : r;
-  const bool bad = slot < -1 || (slot >= 0 && (b < 0 || b >= A.batch || slot >= A.table_ld * A.pool.page_size ||
+  const bool bad = slot < -1 || (slot >= 0 && (b < 0 || b >= A.batch || slot >= A.table_cols * A.pool.page_size ||
                                                ((A.slot_pos || A.mass) && slot >= A.track_ld)));
   if (bad && tid == 0) kv_error(A.bad, KV_ERR_ROW);
   const bool live = slot >= 0 && !bad;
@@ -227,7 +227,7 @@ __global__ void __launch_bounds__(EV_THREADS, 2) kv_evict_select_kernel(const Kv
   __syncthreads();
   kv_pdl_enter();
   bool bad;
-  const int len = (int)kv_len(A.lens[b], min(A.table_ld * A.pool.page_size, A.track_ld), &bad);
+  const int len = (int)kv_len(A.lens[b], min(A.table_cols * A.pool.page_size, A.track_ld), &bad);
   if (bad && tid == 0) kv_error(A.bad, KV_ERR_LEN);
   const int keep = A.keep, new_len = min(len, keep);
   const int share = (int)(((int64_t)len + CL - 1) / CL), s0 = min(len, part * share), n = min(len, s0 + share) - s0;
@@ -512,7 +512,7 @@ cudaError_t kv_evict_init_device() {
 }
 
 cudaError_t kv_evict(const KvEvictArgs& a, int* launches, cudaStream_t s) {
-  const int64_t most = std::min(a.track_ld, a.table_ld * a.pool.page_size);  // slots a sequence may have
+  const int64_t most = std::min(a.track_ld, a.table_cols * a.pool.page_size);  // slots a sequence may have
   const int64_t pairs = a.batch * a.pool.hkv;
   // more CTAs per pair while each has over eight slots a thread and SMs are left (two
   // barriers of the cluster per digit cost what a CTA alone needs for about as many)

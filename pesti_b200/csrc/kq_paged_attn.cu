@@ -147,7 +147,7 @@ __device__ __forceinline__ void tma_load_5d(void* dst, const CUtensorMap* map, i
 
 // Slots a sequence uses: none where its block table (or the tracked slots) cannot hold them.
 __device__ __forceinline__ int pa_len(const KvAttnArgs& A, int64_t b, bool* bad) {
-  int64_t most = A.table_ld * A.pool.page_size;
+  int64_t most = A.table_cols * A.pool.page_size;
   if (A.mass || A.slot_pos) most = min(most, A.track_ld);
   return (int)kv_len(A.lens[b], most, bad);
 }
@@ -818,7 +818,7 @@ template <int HD, int NS>
 cudaError_t launch_attn(const PaParams& P, const KvMaps& maps, int num_sms, cudaStream_t s) {
   using C = PaCfg<HD, NS>;
   const KvAttnArgs& a = P.a;
-  const int64_t tiles = a.batch * a.pool.hkv * ((a.table_ld * a.pool.page_size + PA_TILE - 1) / PA_TILE);
+  const int64_t tiles = a.batch * a.pool.hkv * ((a.table_cols * a.pool.page_size + PA_TILE - 1) / PA_TILE);
   const unsigned grid = (unsigned)std::min<int64_t>(std::min<int64_t>(C::CTAS * num_sms, C::PARTS), tiles);
   return launch_pdl(kv_attn_kernel<HD, NS>, dim3(grid), dim3(C::THREADS), C::END, s, maps.k, maps.v, P);
 }
@@ -874,7 +874,7 @@ cudaError_t kv_attention(const KvAttnArgs& a, const KvMaps& maps, int* launches,
   if (e != cudaSuccess) return e;
   *launches = 1;
   if (!a.mass) return e;
-  const int64_t most = std::min(a.track_ld, a.table_ld * a.pool.page_size);
+  const int64_t most = std::min(a.track_ld, a.table_cols * a.pool.page_size);
   const unsigned chunks = (unsigned)std::min<int64_t>((most + 511) / 512, 64);
   e = launch_pdl(kv_mass_kernel, dim3(chunks, (unsigned)a.pool.hkv, (unsigned)a.batch), dim3(256), 0, s, P);
   *launches += e == cudaSuccess;

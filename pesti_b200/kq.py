@@ -71,7 +71,7 @@ EXPORTED_SYMBOLS = (
     "kq_dec_swiglu", "kq_dec_add", "kq_dec_embed", "kq_dec_norm_linear", "kq_dec_swiglu_linear",
     "kq_dec_residual_linear", "kq_dec_norm_linear_batch", "kq_dec_residual_linear_batch", "kq_dec_rope_attention",
     "kq_dec_tp_partial_linear", "kq_dec_tp_reduce_linear",
-    "kq_kv_create", "kq_kv_destroy", "kq_kv_append", "kq_kv_append_tracked", "kq_kv_attention_scratch", "kq_kv_attention",
+    "kq_kv_create", "kq_kv_destroy", "kq_kv_set_table_cols", "kq_kv_append", "kq_kv_append_tracked", "kq_kv_attention_scratch", "kq_kv_attention",
     "kq_kv_rope_attention", "kq_kv_evict_scratch", "kq_kv_evict", "kq_dec_sample",
     "kq_step_create", "kq_step_linear", "kq_step_attention", "kq_step_run", "kq_step_trace", "kq_step_destroy",
     "kq_gguf_open", "kq_gguf_close", "kq_gguf_tensor_count", "kq_gguf_find_tensor", "kq_gguf_tensor_info",

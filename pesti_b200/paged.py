@@ -21,6 +21,7 @@ def _bind(lib: ctypes.CDLL) -> ctypes.CDLL:
     sig = {
         "kq_kv_create": ([P, P, P, I64, I64, I, I, I, ctypes.POINTER(P)], I),
         "kq_kv_destroy": ([P], I),
+        "kq_kv_set_table_cols": ([P, I64], I),
         "kq_kv_append": ([P, P, I64, I64, I, P, P, P, P, I64, I64, F, P, I64, P, I64], I),
         "kq_kv_append_tracked": ([P, P, I64, I64, I, P, P, P, P, I64, I64, F, P, I64, P, P, I64], I),
         "kq_kv_attention_scratch": ([P, I64, I, I64], Z),
@@ -62,7 +63,7 @@ class PagedCache:
         h = ctypes.c_void_p()
         ctx.check(self.lib.kq_kv_create(ctx.handle, k.data_ptr(), v.data_ptr(), self.pages, page_ld,
                                         self.page_size, self.kv_heads, self.head_dim, ctypes.byref(h)), "kq_kv_create")
-        self.handle = h
+        self.handle, self._cols = h, 0
         self._append, self._attention = self.lib.kq_kv_append_tracked, self.lib.kq_kv_attention
         self._rope_attention = self.lib.kq_kv_rope_attention
 
@@ -78,6 +79,17 @@ class PagedCache:
             pass
         raise _invalid(f"{name}: {t.dtype} {tuple(t.shape)} strides {t.stride()} on {t.device}; "
                        f"{rows if rows >= 0 else 'any'} rows of {dtype} on {self.device} are wanted")
+
+    def _table(self, t, batch: int = -1):
+        """The row stride of a block table, which may be part of a wider one:
+        its own width is what bounds the calls that follow."""
+        ld, cols = self._rows(t, "table", self._types[1], batch), t.shape[1]
+        if cols != self._cols:
+            if cols == 0:
+                raise _invalid("table: no columns")
+            self.ctx.check(self.lib.kq_kv_set_table_cols(self.handle, cols), "kq_kv_set_table_cols")
+            self._cols = cols
+        return ld
 
     def _vector(self, t, name: str, n: int):
         """The address of n contiguous int32."""
@@ -130,7 +142,7 @@ class PagedCache:
         slots' mass starts at 0 (without it a slot used before keeps the weight
         of what lay there), and their positions go to slot_pos."""
         f32, i32 = self._types
-        ld, table_ld = self._rows(qkv, "qkv", f32), self._rows(table, "table", i32)
+        ld, table_ld = self._rows(qkv, "qkv", f32), self._table(table)
         rows, cols = qkv.shape
         batch, hd = table.shape[0], self.head_dim
         heads = cols // hd - 2 * self.kv_heads
@@ -165,7 +177,7 @@ class PagedCache:
             raise _invalid(f"q rows of {cols} and out rows of {out.shape[1]} for heads of {self.head_dim}")
         m, track = (None, 0) if mass is None else self._track(mass, "mass", f32, batch)
         rc = self._attention(self.handle, q.data_ptr(), q_ld, out.data_ptr(), out_ld, batch, heads, table.data_ptr(),
-                             self._rows(table, "table", i32, batch), self._vector(lens, "lens", batch), m, track,
+                             self._table(table, batch), self._vector(lens, "lens", batch), m, track,
                              *self._scratch(scratch))
         if rc:
             self.ctx.check(rc, "kq_kv_attention")
@@ -189,7 +201,7 @@ class PagedCache:
         if slot_pos is not None:
             p, track = self._track(slot_pos, "slot_pos", i32, batch, track)
         rc = self._rope_attention(self.handle, qkv.data_ptr(), ld, out.data_ptr(), out_ld, batch, heads,
-                                  table.data_ptr(), self._rows(table, "table", i32, batch),
+                                  table.data_ptr(), self._table(table, batch),
                                   self._vector(lens, "lens", batch),
                                   None if pos is None else self._vector(pos, "pos", batch), theta, m, p, track,
                                   *self._scratch(scratch))
@@ -209,7 +221,7 @@ class PagedCache:
         po, _ = self._track(pos_out, "pos_out", i32, batch, track)
         sp, sb = self._scratch(scratch)
         self.ctx.check(self.lib.kq_kv_evict(
-            self.handle, batch, table.data_ptr(), self._rows(table, "table", i32), self._vector(lens, "lens", batch),
+            self.handle, batch, table.data_ptr(), self._table(table), self._vector(lens, "lens", batch),
             self._vector(lens_out, "lens_out", batch), m, p, mo, po, track,
             None if recent_from is None else self._vector(recent_from, "recent_from", batch), keep, sp, sb), "kq_kv_evict")
 

@@ -8,7 +8,7 @@ import torch
 
 from pesti_b200 import decoder as dec
 from pesti_b200 import kq, paged, synthetic
-from test_gpu_paged import DEV, TOL_OUT, Setup, keep_of, status, turn
+from test_gpu_paged import DEV, TOL_OUT, Setup, far, keep_of, status, turn
 from test_gpu_serving import LLAMA_TINY
 
 pytestmark = pytest.mark.gpu
@@ -165,3 +165,114 @@ def test_append_checks_the_tracked_slots(gpu_ctx):
     assert status(s.cache.append, qkv, s.table, slots, theta=1e4, mass=mass, slot_pos=spos) == bad
     assert status(s.cache.append, qkv, s.table, slots, theta=1e4, mass=mass.double()) == bad
     assert status(s.cache.append, qkv, s.table, slots, theta=1e4, mass=mass[:1]) == bad
+
+
+# ---- block tables cut out of wider ones -------------------------------------------------------
+
+
+@pytest.mark.parametrize("first", [0, 2])
+def test_a_narrowed_table_bounds_lengths_and_slots_by_its_own_width(gpu_ctx, first):
+    """Three columns of a table of ten whose other entries name pages that hold other rows."""
+    hd, hq, hkv, page, cols = 64, 4, 2, 16, 3
+    full = cols * page
+    s = Setup(gpu_ctx, [full, 20, full], hq, hkv, hd, page, seed=31, spare=4)
+    s.k.nan_to_num_(3.0)
+    s.v.nan_to_num_(3.0)
+    named = torch.zeros(s.pages, dtype=torch.bool)
+    for b, n in enumerate(s.lens_h):
+        named[s.table[b, :-(-n // page)].long().cpu()] = True
+    spare = torch.nonzero(~named)[0].int().to(DEV)
+    wide = spare.repeat(3, 10)
+    wide[:, first:first + cols] = s.table[:, :cols].clamp(0, s.pages - 1)
+    wide[1, first + 2:first + cols] = spare
+    table = wide[:, first:first + cols]
+    assert not table.is_contiguous()
+    qkv = torch.randn((3, (hq + 2 * hkv) * hd), generator=s.g, device=DEV)
+    q = qkv[:, :hq * hd].contiguous()
+    out = torch.full((3, hq * hd), 7.0, device=DEV)
+    ld = 10 * page
+    mass, spos = torch.rand((3, hkv, ld), generator=s.g, device=DEV), torch.zeros((3, hkv, ld), dtype=torch.int32, device=DEV)
+    scratch, es = s.cache.scratch(3, hq, ld), s.cache.evict_scratch(3, ld)
+    lens = torch.tensor([full + 1, 20, full], dtype=torch.int32, device=DEV)
+    k0, v0, m0 = s.k.clone(), s.v.clone(), mass.clone()
+    torch.cuda.synchronize()
+
+    s.cache.attention(q, table, lens, out, scratch)
+    assert status(gpu_ctx.synchronize) == kq.KQ_ERR_INVALID_ARG
+    s.lens_h = [0, 20, full]
+    ref, _ = s.reference(q.view(3, hq, hd))
+    assert far(out.view(3, hq, hd), ref, float(s.v.abs().max())) <= TOL_OUT
+    assert not out[0].any()
+
+    slots, seqs = torch.tensor([full, 5], dtype=torch.int32, device=DEV), torch.tensor([0, 1], dtype=torch.int32, device=DEV)
+    torch.cuda.synchronize()
+    s.cache.append(qkv[:2], table, slots, theta=1e4, seqs=seqs)
+    assert status(gpu_ctx.synchronize) == kq.KQ_ERR_INVALID_ARG
+    at = int(table[1, 0])
+    k0[at, :, 5], v0[at, :, 5] = s.k[at, :, 5], s.v[at, :, 5]
+    assert torch.equal(s.k, k0) and torch.equal(s.v, v0)
+    assert torch.equal(v0[at, :, 5], qkv[1].view(-1, hd)[hq + hkv:].half())
+
+    s.cache.rope_attention(qkv, table, lens, out, scratch, theta=1e4, mass=mass, slot_pos=spos)
+    assert status(gpu_ctx.synchronize) == kq.KQ_ERR_INVALID_ARG
+    for b, n in ((1, 20), (2, full)):
+        at, r = int(table[b, (n - 1) // page]), (n - 1) % page
+        k0[at, :, r], v0[at, :, r] = s.k[at, :, r], s.v[at, :, r]
+        assert torch.equal(v0[at, :, r], qkv[b].view(-1, hd)[hq + hkv:].half())
+    assert torch.equal(s.k, k0) and torch.equal(s.v, v0)
+    assert not out[0].any() and torch.equal(mass[0], m0[0])
+
+    lens2, m2, p2 = torch.zeros_like(lens), mass.clone(), spos.clone()
+    torch.cuda.synchronize()
+    s.cache.evict(table, lens, lens2, mass, spos, m2, p2, 10, es)
+    assert status(gpu_ctx.synchronize) == kq.KQ_ERR_INVALID_ARG
+    assert lens2.tolist() == [full + 1, 10, 10]
+    ids = table[0].long()
+    assert torch.equal(s.k[ids], k0[ids]) and torch.equal(s.k[spare.long()], k0[spare.long()])
+
+    # the next call takes the width of its own table again
+    s.lens_h = [20, 1]
+    two = torch.tensor(s.lens_h, dtype=torch.int32, device=DEV)
+    torch.cuda.synchronize()
+    s.cache.attention(q[:2], s.table[:2], two, out[:2], scratch)
+    gpu_ctx.synchronize()
+    assert far(out[:2].view(2, hq, hd), s.reference(q[:2].view(2, hq, hd))[0], float(s.v.abs().max())) <= TOL_OUT
+
+
+def test_a_narrowed_table_is_captured_with_its_width(gpu_ctx):
+    """Two graphs over one handle, one with the whole table and one with a part of it."""
+    hd, hq, hkv, page = 64, 2, 2, 16
+    s = Setup(gpu_ctx, [70, 30], hq, hkv, hd, page, seed=32)
+    part = s.table[:, :2]
+    q = torch.randn((2, hq * hd), generator=s.g, device=DEV)
+    outs = [torch.empty_like(q) for _ in range(2)]
+    scratch = s.cache.scratch(2, hq)
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    gpu_ctx.set_stream(stream)
+    try:
+        s.cache.attention(q, s.table, s.lens, outs[0], scratch)
+        gpu_ctx.synchronize()
+        graphs = []
+        for table, out in zip((s.table, part), outs):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=stream):
+                s.cache.attention(q, table, s.lens, out, scratch)
+            graphs.append(g)
+        ref, _ = s.reference(q.view(2, hq, hd))
+        for k in (0, 1, 0):
+            outs[k].fill_(9.0)
+            torch.cuda.synchronize()
+            with torch.cuda.stream(stream):
+                graphs[k].replay()
+            if k:
+                assert status(gpu_ctx.synchronize) == kq.KQ_ERR_INVALID_ARG
+            else:
+                gpu_ctx.synchronize()
+            want = ref.clone()
+            if k:
+                want[0] = 0.0  # 70 slots do not fit two pages of 16
+            assert far(outs[k].view(2, hq, hd), want, 5) <= TOL_OUT
+        del graphs, g
+    finally:
+        gpu_ctx.set_stream(None)
