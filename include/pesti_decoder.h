@@ -198,7 +198,8 @@ int kq_kv_set_table_cols(kq_kv *kv, int64_t cols);
  * cache: row r goes to slot slots[r] of sequence seqs[r] (NULL: sequence r), k
  * turned to position pos[r] (NULL: the slot) as in kq_dec_rope_append, with
  * the angle reduced in 64 bits and k exact to the nearest f32 (the bits that
- * kq_kv_rope_attention stores), k and v rounded to f16.  slots[r] = -1 skips
+ * kq_kv_rope_attention stores), k and v rounded to f16 (past 65504: to
+ * infinities, see kq_kv_attention).  slots[r] = -1 skips
  * the row.  q_out (NULL: not needed; it may be qkv itself with q_ld = ld, else
  * it must not overlap it) receives the turned query heads.  slot_pos [batch][kv_heads][track_ld]
  * (NULL: not kept) receives the position of each written slot.  The slots of
@@ -225,6 +226,9 @@ size_t kq_kv_attention_scratch(const kq_kv *kv, int64_t batch, int heads, int64_
 /* Attention of one token per sequence over slots [0, lens[b]):
  * out[b][h] = softmax(q[b][h] . k^T / sqrt(head_dim)) . v with grouped query
  * heads (q turned already).  lens[b] = 0 is an idle row: out[b] is zero.
+ * Infinite keys count as in the formula: a slot whose score is -inf weighs
+ * nothing; a score of +inf, or nothing but -inf, makes that head's row NaN.  An
+ * infinite value leaves its element of the rows that attend to it infinite or NaN.
  * mass [batch][kv_heads][track_ld] (NULL: not kept; lens[b] <= track_ld)
  * accumulates each slot's attention weight, summed over the group's heads. */
 int kq_kv_attention(kq_kv *kv, const float *q, int64_t q_ld, float *out, int64_t out_ld, int64_t batch, int heads,

@@ -34,6 +34,7 @@
 #include "kq_sm100.cuh"
 
 #include <cuda_fp16.h>
+#include <float.h>
 #include <math.h>
 
 namespace kq {
@@ -483,7 +484,8 @@ __global__ void __launch_bounds__(PaCfg<HD, NS>::THREADS, PaCfg<HD, NS>::CTAS)
       float o[C::KS][4];  // O^T: dims 16 mt + g (+ 8), heads 2c, 2c + 1
 #pragma unroll
       for (int mt = 0; mt < C::KS; ++mt) o[mt][0] = o[mt][1] = o[mt][2] = o[mt][3] = 0.f;
-      float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;  // heads 2c, 2c + 1; the maxima less PA_SHIFT
+      // heads 2c, 2c + 1; the maxima less PA_SHIFT (never -inf: slots of -inf weigh 0 next to it)
+      float m0 = -FLT_MAX, m1 = -FLT_MAX, l0 = 0.f, l1 = 0.f;
 
       for (int t = 0; t < n; ++t, ++it) {
         const int s = it % C::STAGES;
@@ -519,6 +521,17 @@ __global__ void __launch_bounds__(PaCfg<HD, NS>::THREADS, PaCfg<HD, NS>::CTAS)
           }
           auto sum = [&](int i) { return sa[0][i] + sa[1][i] + (sb[0][i] + sb[1][i]); };
           float s00 = sum(0) * xs0, s01 = sum(1) * xs1, s10 = sum(2) * xs0, s11 = sum(3) * xs1;
+          if (isnan(s00) || isnan(s01) || isnan(s10) || isnan(s11)) {
+            // an infinite key element against q's second parts, of either sign or 0: the first parts decide
+            auto decided = [&](float s, int i, float x) {
+              const float first = sa[0][i] + sa[1][i];
+              return isinf(first) ? first * x : s;
+            };
+            s00 = decided(s00, 0, xs0);
+            s01 = decided(s01, 1, xs1);
+            s10 = decided(s10, 2, xs0);
+            s11 = decided(s11, 3, xs1);
+          }
           if (A.mass && h0 + 2 * c < P.gp) {
             float* sp = scores + (bh * A.track_ld + slot0) * P.gp + h0 + 2 * c;
             if (g < rows) *reinterpret_cast<float2*>(sp + (int64_t)g * P.gp) = make_float2(s00, s01);
@@ -543,7 +556,7 @@ __global__ void __launch_bounds__(PaCfg<HD, NS>::THREADS, PaCfg<HD, NS>::CTAS)
           x0 = fmaxf(m0, x0 - PA_SHIFT);
           x1 = fmaxf(m1, x1 - PA_SHIFT);
           if (__any_sync(0xffffffffu, x0 != m0 || x1 != m1)) {
-            const float r0 = ex2(m0 - x0), r1 = ex2(m1 - x1);  // 0 while the old maximum is -inf
+            const float r0 = ex2(m0 - x0), r1 = ex2(m1 - x1);
             m0 = x0;
             m1 = x1;
             l0 *= r0;

@@ -2,6 +2,8 @@
 leaves behind for the next, block tables cut out of wider ones, infinite keys,
 and what the calls do with the sequences that are in order beside one that is
 not.  Definitions and tolerances are those of test_gpu_paged."""
+import math
+
 import numpy as np
 import pytest
 import torch
@@ -276,3 +278,69 @@ def test_a_narrowed_table_is_captured_with_its_width(gpu_ctx):
         del graphs, g
     finally:
         gpu_ctx.set_stream(None)
+
+
+# ---- infinite keys ------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("hd,hq,hkv,page", [(64, 14, 2, 16), (128, 32, 8, 64), (256, 9, 1, 48)])
+def test_infinite_keys_weigh_nothing_or_are_reported_as_nan(gpu_ctx, hd, hq, hkv, page):
+    """A score of -inf takes its slot out; one of +inf, or scores that are all -inf, leave no
+    softmax: NaN, in the rows of that sequence and head alone."""
+    lens = [200, 64, 5000, 16, 70, 3]
+    s = Setup(gpu_ctx, lens, hq, hkv, hd, page, seed=hd)
+    B, G = len(lens), hq // hkv
+    q = torch.randn((B, hkv, G, hd), generator=s.g, device=DEV)
+    q[:, :, :, 3], q[:, :, :, hd - 1] = q[:, :, :, 3].abs() + 0.1, -q[:, :, :, hd - 1].abs() - 0.1
+    q = q.reshape(B, hq * hd).contiguous()
+
+    def put(b, slots, d, x, head=slice(None)):
+        for j in slots:
+            s.k[int(s.table[b, j // page]), head, j % page, d] = x
+
+    inf = float("inf")
+    put(0, [0, 5, 40, 199], 3, -inf)                 # single slots
+    put(0, [77], hd - 1, inf)
+    put(0, [78], 3, -inf)                            # two infinities of one slot that agree
+    put(0, [78], hd - 1, inf)
+    put(1, range(16, 32), 3, -inf)                   # all 16 slots of a warp
+    put(2, range(0, 3000), 3, -inf)                  # the first tiles of a sequence that CTAs share
+    put(3, range(1, 16), 3, -inf)                    # all slots but one
+    put(4, [7], 3, inf, 0)                           # +inf, in one kv head
+    put(5, range(3), 3, -inf, hkv - 1)               # nothing left, in one kv head
+    ld = max(lens)
+    out, mass = torch.empty_like(q), torch.zeros((B, hkv, ld), device=DEV)
+    scratch = s.cache.scratch(B, hq, ld)
+    torch.cuda.synchronize()
+    s.cache.attention(q, s.table, s.lens, out, scratch, mass=mass)
+    gpu_ctx.synchronize()
+    ref, ref_mass = s.reference(q.view(B, hq, hd))
+    got = out.view(B, hq, hd)
+    assert torch.equal(got.isnan(), ref.isnan())
+    assert ref[4, :G].isnan().all() and ref[5, hq - G:].isnan().all() and int(ref.isnan().sum()) == 2 * G * hd
+    vmax = float(s.v.nan_to_num(0).abs().max())
+    assert far(got.nan_to_num(0), ref.nan_to_num(0), vmax) <= TOL_OUT
+    for (b, h), m in ref_mass.items():
+        assert torch.equal(mass[b, h, :len(m)].isnan(), m.isnan())
+        assert float((mass[b, h, :len(m)].nan_to_num(0) - m.nan_to_num(0)).abs().max()) <= TOL_OUT * G
+    plain = torch.empty_like(q)  # without the weights: the same output
+    s.cache.attention(q, s.table, s.lens, plain, scratch)
+    gpu_ctx.synchronize()
+    assert torch.equal(plain.nan_to_num(9), out.nan_to_num(9))
+
+
+def test_a_key_past_the_range_of_f16_is_stored_as_infinite(gpu_ctx):
+    """It takes its slot out, or leaves NaN, as its sign says; the other heads are not touched."""
+    hd, hq, hkv = 64, 2, 2
+    s = Setup(gpu_ctx, [40], hq, hkv, hd, 16, seed=41)
+    qkv = torch.randn((1, 6 * hd), generator=s.g, device=DEV)
+    qkv[0, 9], qkv[0, 2 * hd + 9] = 2.0, -1e6
+    pos, lens = torch.zeros(1, dtype=torch.int32, device=DEV), s.lens
+    out, scratch = torch.empty((1, hq * hd), device=DEV), s.cache.scratch(1, hq)
+    torch.cuda.synchronize()
+    s.cache.rope_attention(qkv, s.table, lens, out, scratch, theta=1e4, pos=pos)
+    gpu_ctx.synchronize()
+    assert float(s.k[int(s.table[0, 2]), 0, 39 - 32, 9]) == -math.inf
+    ref, _ = s.reference(qkv[:, :hq * hd].view(1, hq, hd))  # position 0 turns nothing
+    assert torch.isfinite(ref).all()
+    assert far(out.view(1, hq, hd), ref, float(s.v.nan_to_num(0).abs().max())) <= TOL_OUT
