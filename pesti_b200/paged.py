@@ -77,19 +77,27 @@ class PagedCache:
                 return ld if n > 1 else cols
         except ValueError:  # not a matrix
             pass
-        raise _invalid(f"{name}: {t.dtype} {tuple(t.shape)} strides {t.stride()} on {t.device}; "
-                       f"{rows if rows >= 0 else 'any'} rows of {dtype} on {self.device} are wanted")
+        raise self._no_rows(t, name, dtype, rows)
+
+    def _no_rows(self, t, name: str, dtype, rows: int) -> kq.KqError:
+        return _invalid(f"{name}: {t.dtype} {tuple(t.shape)} strides {t.stride()} on {t.device}; "
+                        f"{rows if rows >= 0 else 'any'} rows of {dtype} on {self.device} are wanted")
 
     def _table(self, t, batch: int = -1):
         """The row stride of a block table, which may be part of a wider one:
         its own width is what bounds the calls that follow."""
-        ld, cols = self._rows(t, "table", self._types[1], batch), t.shape[1]
-        if cols != self._cols:
-            if cols == 0:
-                raise _invalid("table: no columns")
-            self.ctx.check(self.lib.kq_kv_set_table_cols(self.handle, cols), "kq_kv_set_table_cols")
-            self._cols = cols
-        return ld
+        try:
+            n, cols = t.shape
+            ld, inner = t.stride()
+            if cols and t.dtype is self._types[1] and t.get_device() == self.index and (inner == 1 or cols == 1) and (
+                    n == batch or batch < 0):
+                if cols != self._cols:
+                    self.ctx.check(self.lib.kq_kv_set_table_cols(self.handle, cols), "kq_kv_set_table_cols")
+                    self._cols = cols
+                return ld if n > 1 else cols
+        except ValueError:  # not a matrix
+            pass
+        raise self._no_rows(t, "table", self._types[1], batch)
 
     def _vector(self, t, name: str, n: int):
         """The address of n contiguous int32."""
