@@ -221,6 +221,7 @@ class PagedCache:
         """Cut sequences of more than `keep` slots to `keep`: the slots at
         positions >= recent_from[b], then those of the greatest mass.  The
         outputs may be the inputs."""
+        keep = min(keep, 2 ** 31 - 1)  # a greater budget would lose its upper bits on the way
         f32, i32 = self._types
         batch = table.shape[0]
         m, track = self._track(mass, "mass", f32, batch)

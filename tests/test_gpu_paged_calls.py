@@ -344,3 +344,19 @@ def test_a_key_past_the_range_of_f16_is_stored_as_infinite(gpu_ctx):
     ref, _ = s.reference(qkv[:, :hq * hd].view(1, hq, hd))  # position 0 turns nothing
     assert torch.isfinite(ref).all()
     assert far(out.view(1, hq, hd), ref, float(s.v.nan_to_num(0).abs().max())) <= TOL_OUT
+
+
+# ---- budgets past 32 bits ------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("keep", [2 ** 31 - 1, 2 ** 31, 2 ** 32 + 5, 2 ** 63 + 1])
+def test_a_budget_past_32_bits_keeps_everything(gpu_ctx, keep):
+    s = Setup(gpu_ctx, [30, 7], 2, 2, 64, 16, seed=51)
+    m, p = torch.rand((2, 2, 30), device=DEV), torch.arange(30, dtype=torch.int32, device=DEV).expand(2, 2, 30).contiguous()
+    es, lens, k0 = s.cache.evict_scratch(2, 30), torch.zeros_like(s.lens), s.k.clone()
+    m0 = m.clone()
+    torch.cuda.synchronize()
+    s.cache.evict(s.table, s.lens, lens, m, p, m, p, keep, es)
+    gpu_ctx.synchronize()
+    assert lens.tolist() == [30, 7]
+    assert torch.equal(m, m0) and torch.equal(s.k.nan_to_num(7), k0.nan_to_num(7))
