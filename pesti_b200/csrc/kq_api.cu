@@ -1428,7 +1428,8 @@ size_t kq_kv_attention_scratch(const kq_kv* kv, int64_t batch, int heads, int64_
   if (!kv || batch < 1 || batch > 65535 || heads < kv->pool.hkv || heads % kv->pool.hkv ||
       heads / kv->pool.hkv > kq::KV_MAX_GROUP || batch * heads > INT32_MAX || track_len < 0 || track_len > INT32_MAX)
     return 0;
-  return kq::kv_attention_scratch_bytes(batch, heads, kv->pool.hkv, kv->pool.hd, track_len, kv->ctx->num_sms);
+  const size_t n = kq::kv_attention_scratch_bytes(batch, heads, kv->pool.hkv, kv->pool.hd, track_len, kv->ctx->num_sms);
+  return n == SIZE_MAX ? 0 : n;
 }
 
 static int kv_attention_impl(kq_kv* kv, const char* what, bool rope, const float* q, int64_t q_ld, float* out,
@@ -1496,7 +1497,8 @@ int kq_kv_rope_attention(kq_kv* kv, const float* qkv, int64_t ld, float* out, in
 
 size_t kq_kv_evict_scratch(const kq_kv* kv, int64_t batch, int64_t track_ld) {
   if (!kv || batch < 1 || batch > 65535 || track_ld < 1 || track_ld > INT32_MAX) return 0;
-  return kq::kv_evict_scratch_bytes(batch, kv->pool.hkv, track_ld);
+  const size_t n = kq::kv_evict_scratch_bytes(batch, kv->pool.hkv, track_ld);
+  return n == SIZE_MAX ? 0 : n;
 }
 
 int kq_kv_evict(kq_kv* kv, int64_t batch, const int32_t* table, int64_t table_ld, const int32_t* lens,

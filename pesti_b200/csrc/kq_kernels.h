@@ -412,6 +412,7 @@ struct KvAttnArgs {
 };
 // head_dim 64, 128 or 256, 1 to KV_MAX_GROUP query heads per kv head.
 constexpr int KV_MAX_GROUP = 16;
+// (SIZE_MAX where the size is past 2^60; the next one too)
 size_t kv_attention_scratch_bytes(int64_t batch, int hq, int hkv, int hd, int64_t track_len, int num_sms);
 cudaError_t kv_attention(const KvAttnArgs& a, const KvMaps& maps, int* launches, cudaStream_t s);
 struct KvEvictArgs {

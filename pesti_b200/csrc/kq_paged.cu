@@ -504,6 +504,7 @@ cudaError_t kv_append(const KvAppendArgs& a, cudaStream_t s) {
 }
 
 size_t kv_evict_scratch_bytes(int64_t batch, int hkv, int64_t track_ld) {
+  if (kv_too_many(batch * hkv, track_ld, (int64_t)(sizeof(EvictPlan) + 4 * sizeof(int)))) return SIZE_MAX;
   return (size_t)batch * hkv * (sizeof(EvictPlan) + (size_t)evict_list(track_ld) * sizeof(int));
 }
 

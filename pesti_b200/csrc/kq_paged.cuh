@@ -27,6 +27,9 @@ __host__ __device__ __forceinline__ int64_t kv_row(const KvPool& p, int32_t page
   return (int64_t)page * p.page_ld + ((int64_t)head * p.page_size + slot % p.page_size) * p.hd;
 }
 
+// a * b * c past 2^60: scratch that no device holds, and whose size could wrap around.
+inline bool kv_too_many(int64_t a, int64_t b, int64_t c) { return (double)a * (double)b * (double)c > 0x1p60; }
+
 #ifdef __CUDACC__
 __device__ __forceinline__ void kv_pdl_enter() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");

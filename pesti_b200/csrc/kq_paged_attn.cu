@@ -872,6 +872,8 @@ cudaError_t kv_init_device() {
 }
 
 size_t kv_attention_scratch_bytes(int64_t batch, int hq, int hkv, int hd, int64_t track_len, int num_sms) {
+  // the scores alone; the rest is far below 2^60
+  if (kv_too_many(batch * hkv, track_len, (hq / hkv + 1) * (int64_t)sizeof(float))) return SIZE_MAX;
   return PaScratch(batch, hq, hkv, hd, track_len, num_sms).end;
 }
 

@@ -360,3 +360,21 @@ def test_a_budget_past_32_bits_keeps_everything(gpu_ctx, keep):
     gpu_ctx.synchronize()
     assert lens.tolist() == [30, 7]
     assert torch.equal(m, m0) and torch.equal(s.k.nan_to_num(7), k0.nan_to_num(7))
+
+
+# ---- sizes ----------------------------------------------------------------------------------------
+
+
+def test_scratch_sizes_past_64_bits_are_refused(gpu_ctx):
+    """Not a small remainder of them (sizes only: nothing is queued)."""
+    pool = torch.zeros((1, 32768, 16, 64), dtype=torch.float16, device=DEV)
+    cache = paged.PagedCache(gpu_ctx, pool, pool.clone())
+    most = 2 ** 31 - 1
+    bad = kq.KQ_ERR_INVALID_ARG
+    # 65535 x 32768 pairs of 2^31 slots: 2^65 bytes of scores, 2^64 of lists
+    assert status(cache.scratch, 65535, 32768, most) == bad
+    assert status(cache.evict_scratch, 65535, most) == bad
+    n = cache.lib.kq_kv_evict_scratch(cache.handle, 4096, 1 << 20)
+    assert n == 4096 * 32768 * (16 + 4 * (1 << 20))
+    n = cache.lib.kq_kv_attention_scratch(cache.handle, 64, 32768, 1 << 20)
+    assert n > 64 * 32768 * 2 * 4 * (1 << 20)
