@@ -327,9 +327,10 @@ class Decoder:
             self.kv_scratch = cache.scratch(B, self.hq, slots if track else 0)
             self.evict_scratch = cache.evict_scratch(B, slots) if track else None
             self._lens_next = torch.zeros_like(self.lens)
-        sbytes = self.lib.kq_dec_attention_scratch(ctx.handle, B, self.hq, self.hkv, hd, self.max_seq)
-        self.att_scratch = torch.zeros(max(sbytes // 4, 1), device=dev)  # counters start at zero
-        self.att_scratch_bytes = sbytes
+        else:
+            sbytes = self.lib.kq_dec_attention_scratch(ctx.handle, B, self.hq, self.hkv, hd, self.max_seq)
+            self.att_scratch = torch.zeros(max(sbytes // 4, 1), device=dev)  # counters start at zero
+            self.att_scratch_bytes = sbytes
         for L in self.layers:
             for key in ("qkv", "o", "gu", "down"):
                 ctx.reserve(L[key], B)

@@ -378,3 +378,16 @@ def test_scratch_sizes_past_64_bits_are_refused(gpu_ctx):
     assert n == 4096 * 32768 * (16 + 4 * (1 << 20))
     n = cache.lib.kq_kv_attention_scratch(cache.handle, 64, 32768, 1 << 20)
     assert n > 64 * 32768 * 2 * 4 * (1 << 20)
+
+
+def test_a_paged_decoder_holds_no_scratch_of_the_contiguous_attention(gpu_ctx):
+    model = dec.Decoder(LLAMA_TINY, gpu_ctx, 2, 20, max_new=4, seed=5, page_size=16)
+    plain = dec.Decoder(LLAMA_TINY, gpu_ctx, 2, 20, max_new=4, seed=5)
+    model.tokens.copy_(torch.tensor([3, 4], dtype=torch.int32))
+    torch.cuda.synchronize()
+    model.step()
+    gpu_ctx.synchronize()
+    assert torch.isfinite(model.logits).all() and bool(model.logits.abs().max() > 0)
+    assert hasattr(plain, "att_scratch") and not hasattr(model, "att_scratch")
+    model.close()
+    plain.close()
