@@ -391,3 +391,91 @@ def test_a_paged_decoder_holds_no_scratch_of_the_contiguous_attention(gpu_ctx):
     assert hasattr(plain, "att_scratch") and not hasattr(model, "att_scratch")
     model.close()
     plain.close()
+
+
+# ---- the sequences beside one that is out of bounds ------------------------------------------------
+
+
+@pytest.mark.parametrize("what", ["page", "negative", "far page", "len", "negative len"])
+def test_the_other_sequences_are_right_beside_one_out_of_bounds(gpu_ctx, what):
+    """Attention and eviction give them what they give alone, and nothing outside the pages of
+    the sequences is written."""
+    hd, hq, hkv, page, keep = 64, 4, 2, 16, 10
+    s = Setup(gpu_ctx, [40, 20, 33], hq, hkv, hd, page, seed=61)
+    table, lens = s.table.clone(), s.lens.clone()
+    long = what in ("len", "negative len")
+    if long:
+        lens[0] = {"len": table.shape[1] * page + 1, "negative len": -3}[what]
+    else:
+        table[0, 1] = {"page": s.pages, "negative": -1, "far page": 2 ** 31 - 1}[what]
+    q, out = torch.randn((3, hq * hd), generator=s.g, device=DEV), torch.full((3, hq * hd), 7.0, device=DEV)
+    m, p = torch.rand((3, hkv, 48), generator=s.g, device=DEV), torch.zeros((3, hkv, 48), dtype=torch.int32, device=DEV)
+    p += torch.arange(48, dtype=torch.int32, device=DEV)
+    scratch, es = s.cache.scratch(3, hq, 48), s.cache.evict_scratch(3, 48)
+    ref, _ = s.reference(q.view(3, hq, hd))
+    k0, v0, m0, p0 = s.k.clone(), s.v.clone(), m.cpu().numpy(), p.cpu().numpy()
+    old = {(b, h): (s.rows(s.k, b, h, n), s.rows(s.v, b, h, n)) for b, n in enumerate(s.lens_h) for h in range(hkv)}
+    vmax = float(s.v.nan_to_num(0).abs().max())
+    torch.cuda.synchronize()
+    s.cache.attention(q, table, lens, out, scratch)
+    assert status(gpu_ctx.synchronize) == kq.KQ_ERR_INVALID_ARG
+    gpu_ctx.synchronize()  # reported once
+    assert far(out[1:].view(2, hq, hd), ref[1:], vmax) <= TOL_OUT
+    if long:
+        assert not out[0].any()
+    assert torch.equal(s.k.nan_to_num(7), k0.nan_to_num(7)) and torch.equal(s.v.nan_to_num(7), v0.nan_to_num(7))
+
+    lens2, m2, p2 = torch.full_like(lens, -9), torch.full_like(m, 77.0), torch.full_like(p, -77)
+    torch.cuda.synchronize()
+    s.cache.evict(table, lens, lens2, m, p, m2, p2, keep, es)
+    assert status(gpu_ctx.synchronize) == kq.KQ_ERR_INVALID_ARG
+    assert lens2.tolist() == [int(lens[0]) if long else keep, keep, keep]
+    assert np.array_equal(m.cpu().numpy(), m0) and np.array_equal(p.cpu().numpy(), p0)
+    if long:
+        assert (m2[0] == 77).all() and (p2[0] == -77).all()
+    mine = torch.zeros(s.pages, dtype=torch.bool, device=DEV)
+    for b in (1, 2) if long else (0, 1, 2):
+        ids = table[b, :-(-s.lens_h[b] // page)].long()
+        mine[ids[(ids >= 0) & (ids < s.pages)]] = True
+    for pool, before in ((s.k, k0), (s.v, v0)):
+        assert torch.equal(pool[~mine].nan_to_num(7), before[~mine].nan_to_num(7))
+    for b in (1, 2):
+        for h in range(hkv):
+            src = keep_of(m0[b, h, :s.lens_h[b]], p0[b, h, :s.lens_h[b]], 1 << 40, keep)
+            assert np.array_equal(m2[b, h, :keep].cpu().numpy(), m0[b, h, src])
+            assert np.array_equal(p2[b, h, :keep].cpu().numpy(), p0[b, h, src])
+            assert (m2[b, h, keep:] == 77).all() and (p2[b, h, keep:] == -77).all()
+            for pool, rows in zip((s.k, s.v), old[b, h]):
+                assert torch.equal(s.rows(pool, b, h, keep), rows[torch.from_numpy(src).to(DEV)])
+
+    # and the next valid call is right for every sequence
+    for pool, before in ((s.k, k0), (s.v, v0)):
+        pool.copy_(before)
+    torch.cuda.synchronize()
+    s.cache.attention(q, s.table, s.lens, out, scratch)
+    gpu_ctx.synchronize()
+    assert far(out.view(3, hq, hd), ref, vmax) <= TOL_OUT
+
+
+@pytest.mark.parametrize("what", ["slot", "far slot", "seq", "negative seq", "page"])
+def test_the_other_rows_are_appended_beside_one_out_of_bounds(gpu_ctx, what):
+    hd, hq, hkv, page = 64, 2, 2, 16
+    s = Setup(gpu_ctx, [40, 20], hq, hkv, hd, page, seed=62)
+    table = s.table[:, :3].contiguous()
+    qkv = torch.randn((3, 6 * hd), generator=s.g, device=DEV)
+    slots = torch.tensor([5, {"slot": 48, "far slot": -2, "page": 17}.get(what, 0), 19], dtype=torch.int32, device=DEV)
+    seqs = torch.tensor([0, {"seq": 2, "negative seq": -1}.get(what, 0), 1], dtype=torch.int32, device=DEV)
+    if what == "page":
+        table[0, 1] = s.pages
+    k0, v0 = s.k.clone(), s.v.clone()
+    torch.cuda.synchronize()
+    s.cache.append(qkv, table, slots, theta=1e4, seqs=seqs)
+    assert status(gpu_ctx.synchronize) == kq.KQ_ERR_INVALID_ARG
+    rows = qkv.view(3, 3 * hkv, hd)
+    want = turn(rows[:, hq:hq + hkv], slots, 1e4).half()
+    for i, (b, t) in ((0, (0, 5)), (2, (1, 19))):
+        at = int(s.table[b, t // page])
+        k0[at, :, t % page], v0[at, :, t % page] = want[i], rows[i, hq + hkv:].half()
+    assert torch.equal(s.v.nan_to_num(7), v0.nan_to_num(7))
+    # the two roundings of a key differ from one at 1e-7 of the elements
+    assert int((s.k.nan_to_num(7) != k0.nan_to_num(7)).sum()) <= 1
