@@ -479,3 +479,27 @@ def test_the_other_rows_are_appended_beside_one_out_of_bounds(gpu_ctx, what):
     assert torch.equal(s.v.nan_to_num(7), v0.nan_to_num(7))
     # the two roundings of a key differ from one at 1e-7 of the elements
     assert int((s.k.nan_to_num(7) != k0.nan_to_num(7)).sum()) <= 1
+
+
+# ---- far positions -----------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("hd,hq,hkv", [(64, 14, 2), (128, 32, 8), (256, 9, 1)])
+def test_rotated_attention_is_as_exact_at_far_positions(gpu_ctx, hd, hq, hkv):
+    """A turned q element is off by four roundings (scale, cosine and sine, a product, the sum) of
+    its pair's length, sqrt(2) of the element on average: 5.7 x 2^-24 of it.  With sum |q_i k_i| /
+    sqrt(hd) about 11 at 128 and 15 at 256, a score by 15 x 3.4e-7 = 5.1e-6 more than the 1.1e-5 of
+    a given q, an output by twice the sum: 3.2e-5, and a quarter on top for the largest of the
+    rows.  An f32 angle would be off by 4e-3 here."""
+    lens = [40, 700, 1, 2049, 130]
+    s = Setup(gpu_ctx, lens, hq, hkv, hd, 16, seed=81)
+    B = len(lens)
+    qkv = 1.5 * torch.randn((B, (hq + 2 * hkv) * hd), generator=s.g, device=DEV)
+    pos = torch.randint(90000, 131072, (B,), generator=s.g, device=DEV).int()
+    out, scratch = torch.empty((B, hq * hd), device=DEV), s.cache.scratch(B, hq)
+    torch.cuda.synchronize()
+    s.cache.rope_attention(qkv, s.table, s.lens, out, scratch, theta=5e5, pos=pos)
+    gpu_ctx.synchronize()
+    q = turn(qkv.view(B, hq + 2 * hkv, hd)[:, :hq], pos, 5e5)
+    ref, _ = s.reference(q)
+    assert far(out.view(B, hq, hd), ref, float(s.v.nan_to_num(0).abs().max())) <= 4e-5
