@@ -79,11 +79,12 @@ __global__ void __launch_bounds__(AP_THREADS, 8) kv_append_kernel(const KvAppend
   // q and k heads in quads of pairs (q only where it is wanted); the first loads come
   // before the row's place is known
   const float* row = A.qkv + r * A.ld;
-  const int quads = half / 4, first = A.q_out ? 0 : A.hq * quads, end = r < A.rows ? (A.hq + hkv) * quads : 0;
+  const int quads = half / 4, log2_quads = 31 - __clz(quads);  // of a head: 8, 16 or 32
+  const int first = A.q_out ? 0 : A.hq * quads, end = r < A.rows ? (A.hq + hkv) * quads : 0;
   float4 x, y;
   auto load = [&](int e) {
     if (e >= end) return;
-    const float* p = row + (int64_t)(e / quads) * hd + 4 * (e % quads);
+    const float* p = row + (int64_t)(e >> log2_quads) * hd + 4 * (e & (quads - 1));
     x = load4(p, vec_in);
     y = load4(p + half, vec_in);
   };
@@ -119,7 +120,7 @@ __global__ void __launch_bounds__(AP_THREADS, 8) kv_append_kernel(const KvAppend
   __half* vc = static_cast<__half*>(A.pool.v) + row0;
   for (int e = first + tid; e < end; e += TPR) {
     if (e != first + tid) load(e);
-    const int head = e / quads, i = 4 * (e % quads);
+    const int head = e >> log2_quads, i = 4 * (e & (quads - 1));
     const float4 c = turn_c[i / 4], s = turn_s[i / 4];
     if (head < A.hq) {
       const float4 a = make_float4(x.x * c.x - y.x * s.x, x.y * c.y - y.y * s.y, x.z * c.z - y.z * s.z,
@@ -143,7 +144,7 @@ __global__ void __launch_bounds__(AP_THREADS, 8) kv_append_kernel(const KvAppend
   }
   if (row0 < 0) return;
   for (int e = tid; e < hkv * (hd / 4); e += TPR) {
-    const int h = e / (hd / 4), i = 4 * (e - h * (hd / 4));
+    const int h = e >> (log2_quads + 1), i = 4 * (e & (2 * quads - 1));
     *reinterpret_cast<uint2*>(vc + h * head_ld + i) = halves(load4(row + (int64_t)(A.hq + hkv + h) * hd + i, vec_in));
   }
   for (int h = tid; h < hkv; h += TPR) {
