@@ -519,19 +519,13 @@ __global__ void __launch_bounds__(PaCfg<HD, NS>::THREADS, PaCfg<HD, NS>::CTAS)
               pa_mma(sb[kk & 1], a, f.z, f.w);
             }
           }
-          auto sum = [&](int i) { return sa[0][i] + sa[1][i] + (sb[0][i] + sb[1][i]); };
+          // An infinite key element meets q's second parts with either sign or as 0: the first
+          // parts decide (by select: 32 x 2049 slots of 128 / 8 heads take 75.3 us, with a branch 77.0)
+          auto sum = [&](int i) {
+            const float first = sa[0][i] + sa[1][i];
+            return isinf(first) ? first : first + (sb[0][i] + sb[1][i]);
+          };
           float s00 = sum(0) * xs0, s01 = sum(1) * xs1, s10 = sum(2) * xs0, s11 = sum(3) * xs1;
-          if (isnan(s00) || isnan(s01) || isnan(s10) || isnan(s11)) {
-            // an infinite key element against q's second parts, of either sign or 0: the first parts decide
-            auto decided = [&](float s, int i, float x) {
-              const float first = sa[0][i] + sa[1][i];
-              return isinf(first) ? first * x : s;
-            };
-            s00 = decided(s00, 0, xs0);
-            s01 = decided(s01, 1, xs1);
-            s10 = decided(s10, 2, xs0);
-            s11 = decided(s11, 3, xs1);
-          }
           if (A.mass && h0 + 2 * c < P.gp) {
             float* sp = scores + (bh * A.track_ld + slot0) * P.gp + h0 + 2 * c;
             if (g < rows) *reinterpret_cast<float2*>(sp + (int64_t)g * P.gp) = make_float2(s00, s01);
