@@ -21,7 +21,7 @@ namespace cg = cooperative_groups;
 // by the row's bytes: f32 in, f32 q and f16 k, v out.  Many small CTAs hide the chain
 // slot - page - row better than several steps' loads in flight: 4099 rows of 32 / 8
 // heads of 128 took 33.2 us with one step and eight CTAs per SM, 38.9 with four steps
-// and four (a call takes 36.6 us, 5040 GB/s, since keys are exact; 35.8 with f32 sums).
+// and four (34.9 us, 5290 GB/s, since keys are exact and heads found by shifts).
 constexpr int AP_THREADS = 256, AP_MAX_HALF = 128;
 
 // Four floats at p, in one access where `vec` (p is then 16-byte aligned).
@@ -48,7 +48,7 @@ __device__ __forceinline__ uint2 halves(float4 v) { return make_uint2(pair_bits(
 // where its error could round another way (one pair in 100) by exact_dot2.  The error:
 // c, s, the product rounded by itself and the sum each add 2^-24 of what they round,
 // together at most 3 x 2^-24 of the two products.  lo: what f32 leaves of the cosines,
-// and `half` behind that of the sines.  (4099 rows: a call 36.6 us; 37.6 by exact_dot2 alone.)
+// and `half` behind that of the sines.  (4099 rows: 1.0 us less of 37.6 than by exact_dot2 alone.)
 __device__ __forceinline__ void turn_keys(float2 x, float2 y, float2 c, float2 s, const float* lo, int half,
                                           uint32_t& a, uint32_t& b) {
   constexpr float E = 0x1.8p-23f;
@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(AP_THREADS, 8) kv_append_kernel(const KvAppend
 // stay in shared memory (up to EV_PIECE slots a CTA; longer shares go piece by
 // piece).  A second kernel moves the rows: it is bound by them, the first by the
 // latency of its passes.  Measured: 8 sequences of 2113 to 2048 slots, 8 heads of 128,
-// 13.8 us; 4 of up to 32,771 to 4096 30.9 us, of which the rows take about half (33 MB
+// 13.7 us; 4 of up to 32,771 to 4096 31.4 us, of which the rows take about half (33 MB
 // read, as much written).
 constexpr int EV_THREADS = 512, EV_BINS = 2048, EV_PIECE = 20480, EV_LOADS = 8, EV_MAX_CLUSTER = 8;
 constexpr size_t EV_SMEM = (size_t)EV_PIECE * 4;

@@ -26,9 +26,9 @@
 // carried times 2^14, which keeps its second part clear of the subnormals.
 // Groups of 9 to 16 heads run a second set of four warps on the same tiles.
 //
-// Measured: 32 sequences of 128 to 4096 slots, 32 / 8 heads of 128, 53.4 us (264 MB:
+// Measured: 32 sequences of 128 to 4096 slots, 32 / 8 heads of 128, 53.6 us (264 MB:
 // 5.0 TB/s over the call, 7.4 in its steady part; 4.5 us go to lengths - table - first
-// tile, about 5 to the join); one of 131,077 slots 91.8 us (5.9 TB/s); one of 2049
+// tile, about 5 to the join); one of 131,077 slots 91.4 us (5.9 TB/s); one of 2049
 // rotated, appended and attended 11.7 us; one of 17, 14 / 2 heads of 64, 4.2 us.
 #include "kq_paged.cuh"
 #include "kq_sm100.cuh"

@@ -24,8 +24,8 @@
 //  * the draw: sums per thread over consecutive tokens, and one thread walks the
 //    stretch that holds it.
 // Measured: one row of 151,936 with every filter 11.7 us, 32 rows of 128,256 under
-// top-p 38.0 us (issue slots 49% busy: 139 warp instructions per 32 tokens, 60 of
-// them for the shared atomics of the bins; one read of the logits would take 2.5), 64 rows of 151,936 with settings of their own 54.3 us.
+// top-p 38.1 us (issue slots 49% busy: 139 warp instructions per 32 tokens, 60 of
+// them for the shared atomics of the bins; one read of the logits would take 2.5), 64 rows of 151,936 with settings of their own 55.0 us.
 #include "kq_common.cuh"
 #include "kq_kernels.h"
 
